@@ -16,6 +16,8 @@ ACT_RELU = 1
 ACT_TANH, ACT_SIGMOID, ACT_ELU, ACT_SOFTPLUS, ACT_SELU, ACT_SWISH = 2, 3, 4, 5, 6, 7
 ACT_GELU, ACT_SOFTSIGN, ACT_EXPONENTIAL, ACT_HARD_SIGMOID = 8, 9, 10, 11
 
+DTYPE_F32, DTYPE_BF16, DTYPE_F16 = 0, 1, 2
+
 MATMUL_MODES = {'f32': 0, 'split3': 1, 'split2': 2, 'bf16': 3}
 
 i32p = C.POINTER(C.c_int32)
@@ -146,6 +148,32 @@ SIGNATURES = {
     'gunet_error_sums_workspace_bytes': (C.c_size_t, [C.c_int64, C.c_int32, C.c_int32]),
     'gunet_error_sums_f32': (C.c_int, [C.c_void_p, C.c_void_p, C.c_int64, C.c_int32, C.c_int32, C.c_void_p,
                                        C.c_void_p, C.c_size_t, C.c_void_p]),
+    'gunet_expert_sort_workspace_bytes': (C.c_size_t, [C.c_int64, C.c_int32, C.c_int32]),
+    'gunet_expert_sort': (C.c_int, [C.c_void_p, C.c_int64, C.c_int32, C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p,
+                                    C.c_void_p, C.c_size_t, C.c_void_p]),
+    'gunet_expert_dispatch': (C.c_int, [C.c_void_p, C.c_int32, C.c_void_p, C.c_void_p, C.c_int64, C.c_int32, C.c_int32,
+                                        C.c_int64, C.c_void_p, C.c_void_p]),
+    'gunet_expert_dispatch_grad': (C.c_int, [C.c_void_p, C.c_int32, C.c_void_p, C.c_int64, C.c_int32, C.c_int64,
+                                             C.c_void_p, C.c_void_p]),
+    'gunet_expert_combine': (C.c_int, [C.c_void_p, C.c_int32, C.c_void_p, C.c_void_p, C.c_int64, C.c_int32, C.c_int64,
+                                       C.c_void_p, C.c_void_p]),
+    'gunet_expert_combine_grad': (C.c_int, [C.c_void_p, C.c_void_p, C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p,
+                                            C.c_int64, C.c_int32, C.c_int32, C.c_int64, C.c_void_p, C.c_void_p,
+                                            C.c_void_p]),
+    'gunet_mxfp4_code_bytes': (C.c_size_t, [C.c_int64, C.c_int64, C.c_int32]),
+    'gunet_mxfp4_scale_bytes': (C.c_size_t, [C.c_int64, C.c_int64, C.c_int32]),
+    'gunet_mxfp4_quantize': (C.c_int, [C.c_void_p, C.c_int32, C.c_int64, C.c_int64, C.c_int32, C.c_void_p, C.c_void_p,
+                                       C.c_void_p]),
+    'gunet_mxfp4_dequantize': (C.c_int, [C.c_void_p, C.c_void_p, C.c_int64, C.c_int64, C.c_int32, C.c_void_p,
+                                         C.c_int32, C.c_void_p]),
+    'gunet_mxfp4_dense_workspace_bytes': (C.c_size_t, [C.c_int64, C.c_int32]),
+    'gunet_mxfp4_dense_forward': (C.c_int, [C.c_void_p, C.c_int32, C.c_int64, C.c_int32, C.c_void_p, C.c_void_p,
+                                            C.c_void_p, C.c_int32, C.c_int32, C.c_void_p, C.c_int32, C.c_void_p,
+                                            C.c_size_t, C.c_void_p]),
+    'gunet_mxfp4_expert_dense_forward': (C.c_int, [C.c_void_p, C.c_int32, C.c_void_p, C.c_void_p, C.c_int64, C.c_int32,
+                                                   C.c_int32, C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int32,
+                                                   C.c_int32, C.c_void_p, C.c_int32, C.c_void_p, C.c_size_t,
+                                                   C.c_void_p]),
     'gunet_profile_enable': (C.c_int, [C.c_int]),
     'gunet_profile_collect': (C.c_int, [C.POINTER(F64xP), C.POINTER(I64xP), C.POINTER(F64xP)]),
     'gunet_profile_class_name': (C.c_char_p, [C.c_int]),

@@ -1,0 +1,134 @@
+"""Rows sorted by expert and back (no counterpart in the reference): the learned form of its quadrant lists.
+
+A router names top_k experts for every row (token).  `expert_plan` sorts those choices, `expert_dispatch` copies the rows
+into expert order, the experts work on consecutive rows, and `expert_combine` adds their results back with
+the router's weights:
+
+    plan = expert_plan(index, n_experts)               # index int32 [T, k]; -1 = dropped
+    rows = expert_dispatch(x, plan)                    # [T * k, C], expert e at plan.offsets[e]:plan.offsets[e + 1]
+    ...                                                # e.g. mxfp4_expert_dense
+    out = expert_combine(rows, weights, plan)          # weights float32 [T, k]
+
+Unlike the index plans of the city graphs nothing here synchronises or is cached: a router chooses
+anew at every step, and everything can be captured into a HIP graph.  Like the rest of the package the functions record no
+autograd graph: a training step calls the gradients, `expert_combine_grad` and `expert_dispatch_grad`, itself (or from
+an autograd.Function of its own); a tensor that requires a gradient is refused rather than dropped from the graph.
+Tensors may be strided (they are then copied first); all of them on one GPU, whose current stream the work goes to.
+"""
+import torch
+
+from .. import _lib
+from .._lib import call, current_stream, ptr
+
+DTYPES = {torch.float32: _lib.DTYPE_F32, torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_F16}
+
+
+def dtype_code(t, what):
+    code = DTYPES.get(t.dtype)
+    if code is None:
+        raise TypeError(f'{what} must be float32, bfloat16 or float16, got {t.dtype}')
+    return code
+
+
+def checked(t, what, device=None, dtype=None, shape=None):
+    """t as a packed tensor, or a TypeError / ValueError that says what is wrong with it."""
+    if not (isinstance(t, torch.Tensor) and t.is_cuda):
+        raise TypeError(f'{what} must be a CUDA tensor')
+    if device is not None and t.device != device:
+        raise ValueError(f'{what} is on {t.device}, the other tensors are on {device}')
+    if dtype is not None and t.dtype != dtype:
+        raise TypeError(f'{what} must be {dtype}, got {t.dtype}')
+    if shape is not None and tuple(t.shape) != tuple(shape):
+        raise ValueError(f'{what} must have the shape {tuple(shape)}, got {tuple(t.shape)}')
+    if t.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f'{what} requires a gradient: this call records no autograd graph (detach it, or call under '
+                         'torch.no_grad() and use the _grad functions)')
+    return t.contiguous()
+
+
+class ExpertPlan:
+    """offsets int32 [n_experts + 1] (rows of each expert), order int32 [T * k] (flat position t * k + j of each
+    row, -1 behind the last) and slot int32 [T, k] (row of each choice, -1 = dropped)."""
+
+    def __init__(self, offsets, order, slot, n_experts):
+        self.offsets, self.order, self.slot = offsets, order, slot
+        self.n_experts = n_experts
+        self.n_tokens, self.top_k = slot.shape
+        self.device = slot.device
+
+    @property
+    def n_rows(self):
+        return self.n_tokens * self.top_k
+
+
+def expert_plan(expert_index, n_experts):
+    """The order of the choices expert_index int32 [T, k]; a value outside 0 .. n_experts - 1 drops the choice."""
+    index = checked(expert_index, 'expert_index', dtype=torch.int32)
+    if index.dim() != 2 or index.shape[1] < 1:
+        raise ValueError(f'expert_index must be [T, k] with k >= 1, got {tuple(index.shape)}')
+    n_experts = int(n_experts)
+    t, k = index.shape
+    dev = index.device
+    offsets = torch.empty(max(n_experts, 0) + 1, dtype=torch.int32, device=dev)
+    order = torch.empty(t * k, dtype=torch.int32, device=dev)
+    slot = torch.empty((t, k), dtype=torch.int32, device=dev)
+    nbytes = _lib.lib.gunet_expert_sort_workspace_bytes(t, k, n_experts)
+    scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    with torch.cuda.device(dev):
+        call('gunet_expert_sort', ptr(index), t, k, n_experts, ptr(offsets), ptr(order), ptr(slot), ptr(scratch), nbytes,
+             current_stream(dev))
+    return ExpertPlan(offsets, order, slot, n_experts)
+
+
+def _width(t, what, rows):
+    if t.dim() != 2 or t.shape[0] != rows:
+        raise ValueError(f'{what} must be [{rows}, width], got {tuple(t.shape)}')
+    return t.shape[1]
+
+
+def expert_dispatch(x, plan):
+    """x [T, C] -> rows [T * k, C] in expert order (zeros behind the last expert's)."""
+    x = checked(x, 'x', plan.device)
+    width = _width(x, 'x', plan.n_tokens)
+    rows = torch.empty((plan.n_rows, width), dtype=x.dtype, device=x.device)
+    with torch.cuda.device(x.device):
+        call('gunet_expert_dispatch', ptr(x), dtype_code(x, 'x'), ptr(plan.offsets), ptr(plan.slot), plan.n_tokens, plan.top_k,
+             plan.n_experts, width, ptr(rows), current_stream(x.device))
+    return rows
+
+
+def expert_dispatch_grad(grad_rows, plan):
+    """Gradient of expert_dispatch: grad_rows [T * k, C] -> grad_x [T, C]."""
+    g = checked(grad_rows, 'grad_rows', plan.device)
+    width = _width(g, 'grad_rows', plan.n_rows)
+    grad_x = torch.empty((plan.n_tokens, width), dtype=g.dtype, device=g.device)
+    with torch.cuda.device(g.device):
+        call('gunet_expert_dispatch_grad', ptr(g), dtype_code(g, 'grad_rows'), ptr(plan.slot), plan.n_tokens, plan.top_k, width,
+             ptr(grad_x), current_stream(g.device))
+    return grad_x
+
+
+def expert_combine(rows, weights, plan):
+    """out[t] = sum_j weights[t, j] * rows[slot[t, j]]: rows [T * k, C], weights float32 [T, k] -> [T, C]."""
+    rows = checked(rows, 'rows', plan.device)
+    width = _width(rows, 'rows', plan.n_rows)
+    w = checked(weights, 'weights', plan.device, torch.float32, plan.slot.shape)
+    out = torch.empty((plan.n_tokens, width), dtype=rows.dtype, device=rows.device)
+    with torch.cuda.device(rows.device):
+        call('gunet_expert_combine', ptr(rows), dtype_code(rows, 'rows'), ptr(w), ptr(plan.slot), plan.n_tokens, plan.top_k, width,
+             ptr(out), current_stream(rows.device))
+    return out
+
+
+def expert_combine_grad(grad_out, rows, weights, plan):
+    """Gradients of expert_combine: (grad_rows [T * k, C] in the type of rows, grad_weights float32 [T, k])."""
+    rows = checked(rows, 'rows', plan.device)
+    width = _width(rows, 'rows', plan.n_rows)
+    g = checked(grad_out, 'grad_out', plan.device, rows.dtype, (plan.n_tokens, width))
+    w = checked(weights, 'weights', plan.device, torch.float32, plan.slot.shape)
+    grad_rows = torch.empty_like(rows)
+    grad_weights = torch.empty_like(w)
+    with torch.cuda.device(rows.device):
+        call('gunet_expert_combine_grad', ptr(g), ptr(rows), dtype_code(rows, 'rows'), ptr(w), ptr(plan.offsets), ptr(plan.slot),
+             plan.n_tokens, plan.top_k, plan.n_experts, width, ptr(grad_rows), ptr(grad_weights), current_stream(rows.device))
+    return grad_rows, grad_weights

@@ -1,0 +1,153 @@
+"""Dense on microscaled 4-bit weights (no counterpart in the reference): the step below the bf16 matmul mode.
+
+    w4 = mxfp4_quantize(kernel.t())                    # [n_out, k], once
+    y = mxfp4_dense(x, w4, bias, 'relu')               # x is quantised on the way in
+
+or, for a layer that exists already, `Mxfp4Dense.from_dense(dense)`.  Weights of several experts are one tensor [E, n_out, k],
+used by mxfp4_expert_dense on the rows that an expert_plan has sorted.  The format is OCP MXFP4: blocks of 32 columns
+share a power of two, elements are +-0, .5, 1, 1.5, 2, 3, 4, 6 (include/gunet_hip.h has every rule).  For serving: no
+gradients (a tensor that requires one is refused), nothing synchronises, everything can be captured into a HIP graph.
+"""
+import torch
+
+from .. import _lib
+from .._lib import call, current_stream, ptr
+from .expert_ops import DTYPES, checked, dtype_code
+from .hybrid_gnn import _activation_code
+
+BLOCK = 32
+
+
+class Mxfp4Tensor:
+    """A 4-bit matrix [rows, k] or stack of matrices [groups, rows, k]: codes uint8 [groups, rows, blocks, 16] and scales uint8
+    [groups, ceil(blocks / 8), rows, 8], the layout of include/gunet_hip.h."""
+
+    def __init__(self, codes, scales, shape):
+        self.codes, self.scales, self.shape = codes, scales, tuple(shape)
+        self.groups, self.rows, self.k = ((1,) + self.shape)[-3:]
+        self.device = codes.device
+
+    @classmethod
+    def empty(cls, shape, device):
+        if len(shape) not in (2, 3) or shape[-1] < 1:
+            raise ValueError(f'a 4-bit tensor is [rows, k] or [groups, rows, k] with k >= 1, got {tuple(shape)}')
+        groups, rows, k = ((1,) + tuple(shape))[-3:]
+        blocks = -(-k // BLOCK)
+        return cls(torch.empty((groups, rows, blocks, 16), dtype=torch.uint8, device=device),
+                   torch.empty((groups, -(-blocks // 8), rows, 8), dtype=torch.uint8, device=device), shape)
+
+    @classmethod
+    def from_codes(cls, codes, scales, k):
+        """From the row-major form that checkpoints hold: codes uint8 [.., rows, blocks * 16] (two columns a byte, the even one in the
+        low four bits), scales uint8 [.., rows, blocks] (exponent + 127), blocks = ceil(k / 32)."""
+        codes, scales = checked(codes, 'codes', dtype=torch.uint8), checked(scales, 'scales', dtype=torch.uint8)
+        blocks = -(-int(k) // BLOCK)
+        if codes.dim() not in (2, 3) or k < 1 or codes.shape[-1] != blocks * 16:
+            raise ValueError(f'codes must be [.., rows, {blocks * 16}] for k = {k}, got {tuple(codes.shape)}')
+        if tuple(scales.shape) != tuple(codes.shape[:-1]) + (blocks,) or scales.device != codes.device:
+            raise ValueError(f'scales must be {tuple(codes.shape[:-1]) + (blocks,)} on {codes.device}, got {tuple(scales.shape)} on {scales.device}')
+        t = cls.empty(codes.shape[:-1] + (int(k),), codes.device)
+        t.codes.copy_(codes.view(t.codes.shape))
+        if k % BLOCK:                                   # columns behind k: zeros, whatever the padding held
+            used = k % BLOCK
+            t.codes[:, :, -1, (used + 1) // 2:] = 0
+            if used % 2:
+                t.codes[:, :, -1, used // 2] &= 15
+        t.scales.zero_()
+        grouped = torch.nn.functional.pad(scales.view(t.groups, t.rows, blocks), (0, -blocks % 8))
+        t.scales.copy_(grouped.view(t.groups, t.rows, -1, 8).transpose(1, 2))
+        return t
+
+
+def mxfp4_quantize(x):
+    """x float32 / bfloat16 / float16 [rows, k] or [groups, rows, k] -> Mxfp4Tensor."""
+    x = checked(x, 'x')
+    code = dtype_code(x, 'x')
+    t = Mxfp4Tensor.empty(x.shape, x.device)
+    with torch.cuda.device(x.device):
+        call('gunet_mxfp4_quantize', ptr(x), code, t.groups, t.rows, t.k, ptr(t.codes), ptr(t.scales), current_stream(x.device))
+    return t
+
+
+def mxfp4_dequantize(t, dtype=torch.float32):
+    """The values of an Mxfp4Tensor (float16 may overflow or lose the smallest ones)."""
+    if dtype not in DTYPES:
+        raise TypeError(f'dtype must be float32, bfloat16 or float16, got {dtype}')
+    out = torch.empty(t.shape, dtype=dtype, device=t.device)
+    with torch.cuda.device(t.device):
+        call('gunet_mxfp4_dequantize', ptr(t.codes), ptr(t.scales), t.groups, t.rows, t.k, ptr(out), DTYPES[dtype],
+             current_stream(t.device))
+    return out
+
+
+def _operands(x, w, bias, activation, out_dtype, groups_shape):
+    if not isinstance(w, Mxfp4Tensor):
+        raise TypeError('w must be an Mxfp4Tensor')
+    x = checked(x, 'x', w.device)
+    if x.dim() < 1 or x.shape[-1] != w.k:
+        raise ValueError(f'x has {x.shape[-1] if x.dim() else 0} columns, w has {w.k}')
+    if bias is not None:
+        bias = checked(bias, 'bias', w.device, torch.float32, groups_shape + (w.rows,))
+    out_dtype = x.dtype if out_dtype is None else out_dtype
+    if out_dtype not in DTYPES:
+        raise TypeError(f'out_dtype must be float32, bfloat16 or float16, got {out_dtype}')
+    return x, dtype_code(x, 'x'), bias, _activation_code(activation), out_dtype
+
+
+def mxfp4_dense(x, w, bias=None, activation=None, out_dtype=None):
+    """act(q(x) @ w^T + bias): x [.., k] float32 / bfloat16 / float16, w Mxfp4Tensor [n_out, k], bias float32 [n_out];
+    the result [.., n_out] has x's type unless out_dtype names another.  Activations as for Dense."""
+    x, code, bias, act, out_dtype = _operands(x, w, bias, activation, out_dtype, ())
+    if len(w.shape) != 2:
+        raise ValueError(f'w must be [n_out, k], got {w.shape} (mxfp4_expert_dense takes stacks)')
+    rows = x.numel() // w.k
+    out = torch.empty(x.shape[:-1] + (w.rows,), dtype=out_dtype, device=x.device)
+    scratch = torch.empty(_lib.lib.gunet_mxfp4_dense_workspace_bytes(rows, w.k), dtype=torch.uint8, device=x.device)
+    with torch.cuda.device(x.device):
+        call('gunet_mxfp4_dense_forward', ptr(x), code, rows, w.k, ptr(w.codes), ptr(w.scales), ptr(bias), w.rows, act, ptr(out),
+             DTYPES[out_dtype], ptr(scratch), scratch.numel(), current_stream(x.device))
+    return out
+
+
+def mxfp4_expert_dense(x, w, plan, bias=None, activation=None, out_dtype=None, sorted_rows=False):
+    """The experts' Dense layers on the rows of an ExpertPlan: w Mxfp4Tensor [E, n_out, k], bias float32 [E, n_out].
+    x [T, k] holds the tokens (each row is dispatched in its 4-bit form), or with sorted_rows=True
+    x [T * top_k, k] rows in expert order.  Returns [T * top_k, n_out] in expert order, zeros behind the last expert's rows."""
+    x, code, bias, act, out_dtype = _operands(x, w, bias, activation, out_dtype, (getattr(w, 'groups', 0),))
+    if len(w.shape) != 3 or w.groups != plan.n_experts:
+        raise ValueError(f'w must be [{plan.n_experts}, n_out, k], got {w.shape}')
+    if plan.device != x.device:
+        raise ValueError(f'the plan is on {plan.device}, x is on {x.device}')
+    want = plan.n_rows if sorted_rows else plan.n_tokens
+    if x.dim() != 2 or x.shape[0] != want:
+        raise ValueError(f'x must be [{want}, {w.k}], got {tuple(x.shape)}')
+    out = torch.empty((plan.n_rows, w.rows), dtype=out_dtype, device=x.device)
+    scratch = torch.empty(_lib.lib.gunet_mxfp4_dense_workspace_bytes(plan.n_rows, w.k), dtype=torch.uint8, device=x.device)
+    with torch.cuda.device(x.device):
+        call('gunet_mxfp4_expert_dense_forward', ptr(x), code, ptr(plan.offsets), None if sorted_rows else ptr(plan.slot),
+             plan.n_tokens, plan.top_k, plan.n_experts, w.k, ptr(w.codes), ptr(w.scales), ptr(bias), w.rows, act, ptr(out),
+             DTYPES[out_dtype], ptr(scratch), scratch.numel(), current_stream(x.device))
+    return out
+
+
+class Mxfp4Dense:
+    """A Dense layer served from 4-bit weights: the same call, y = activation(x @ kernel + bias)."""
+
+    def __init__(self, units, weights, bias=None, activation=None):
+        if not isinstance(weights, Mxfp4Tensor) or len(weights.shape) != 2 or weights.rows != units:
+            raise ValueError(f'weights must be an Mxfp4Tensor [{units}, in]')
+        self.units, self.weights, self.bias, self.activation = units, weights, bias, activation
+        _activation_code(activation)
+
+    @classmethod
+    def from_dense(cls, dense):
+        """From a hybrid_gnn.Dense that holds its weights: the kernel [in, units] is transposed and quantised, the
+        bias stays float32."""
+        if dense.kernel is None:
+            raise ValueError('the Dense layer has no weights yet')
+        bias = dense.bias.detach().clone() if dense.bias is not None else None
+        return cls(dense.units, mxfp4_quantize(dense.kernel.detach().t()), bias, dense.activation)
+
+    def __call__(self, x, activation=Ellipsis):
+        """activation overrides the layer's own for this call, as in Dense."""
+        return mxfp4_dense(x, self.weights, self.bias, self.activation if activation is Ellipsis else activation)

@@ -367,6 +367,88 @@ int gunet_unet_forward_static_f32(const gunet_plan* plan, const gunet_unet_weigh
                                   float* const edges_out[4], float* global_out, gunet_stream_t stream);
 
 /* ------------------------------------------------------------------------
+ * 2c. Rows sorted by expert, and Dense on 4-bit weights -- no counterpart in the reference
+ *
+ * The learned form of the quadrant lists: a router gives every row (token) top_k expert numbers, the rows go to their
+ * experts' Dense layers and come back weighted.  And the step below GUNET_MATMUL_BF16 for Dense: weights
+ * and activations in blocks of 32 four-bit numbers with a shared power of two.  All functions are asynchronous,
+ * allocate nothing and may be captured into a HIP graph; tensors are packed row-major; results repeat bit for
+ * bit.  They are not part of the profiler's classes.
+ * ------------------------------------------------------------------------ */
+
+/* Element type of the tensors passed as void* (aligned to the type's size; 16-byte aligned rows are faster). */
+#define GUNET_DTYPE_F32 0
+#define GUNET_DTYPE_BF16 1
+#define GUNET_DTYPE_F16 2
+
+/* Stable counting sort of the n = n_tokens * top_k flat positions f = t * top_k + j by expert_index[t][j]
+ * (int32 [n_tokens, top_k]).  A value outside 0 .. n_experts-1 is a dropped choice.
+ *   offsets int32 [n_experts + 1]      rows offsets[e] .. offsets[e+1]-1 belong to expert e
+ *   order   int32 [n]                  flat position of each row, ascending within an expert; -1 behind
+ *                                      offsets[n_experts]
+ *   slot    int32 [n_tokens, top_k]    the inverse: row of each flat position; -1 = dropped
+ * A token may name one expert several times.  n <= 2^31 - 1; n_experts <= 1024 (else GUNET_ERR_UNSUPPORTED).
+ * workspace: 4-byte aligned; gunet_expert_sort_workspace_bytes may be 0, then it may be NULL. */
+size_t gunet_expert_sort_workspace_bytes(int64_t n_tokens, int32_t top_k, int32_t n_experts);
+int gunet_expert_sort(const int32_t* expert_index, int64_t n_tokens, int32_t top_k, int32_t n_experts, int32_t* offsets,
+                      int32_t* order, int32_t* slot, void* workspace, size_t workspace_bytes, gunet_stream_t stream);
+
+/* rows[slot[t][j]] = x[t] for every kept choice, zeros in the rows behind offsets[n_experts]: x [n_tokens, width],
+ * rows [n_tokens * top_k, width], both of type `dtype`.  Outputs may not overlap inputs (here and below). */
+int gunet_expert_dispatch(const void* x, int32_t dtype, const int32_t* offsets, const int32_t* slot, int64_t n_tokens,
+                          int32_t top_k, int32_t n_experts, int64_t width, void* rows, gunet_stream_t stream);
+/* Its gradient: grad_x[t] = sum_j grad_rows[slot[t][j]], float32 sums from j = 0 up, rounded once. */
+int gunet_expert_dispatch_grad(const void* grad_rows, int32_t dtype, const int32_t* slot, int64_t n_tokens, int32_t top_k,
+                               int64_t width, void* grad_x, gunet_stream_t stream);
+
+/* out[t] = sum_j weights[t][j] * rows[slot[t][j]] over the kept choices (0 if there are none): rows [n_tokens * top_k, width]
+ * and out [n_tokens, width] of type `dtype`, weights float32 [n_tokens, top_k].  float32 sums from j = 0 up, rounded once. */
+int gunet_expert_combine(const void* rows, int32_t dtype, const float* weights, const int32_t* slot, int64_t n_tokens,
+                         int32_t top_k, int64_t width, void* out, gunet_stream_t stream);
+/* Its gradient: grad_rows[slot[t][j]] = weights[t][j] * grad_out[t] (zeros in the rows behind offsets[n_experts]), and
+ * grad_weights[t][j] = <grad_out[t], rows[slot[t][j]]> in float32 (0 for a dropped choice). */
+int gunet_expert_combine_grad(const void* grad_out, const void* rows, int32_t dtype, const float* weights,
+                              const int32_t* offsets, const int32_t* slot, int64_t n_tokens, int32_t top_k,
+                              int32_t n_experts, int64_t width, void* grad_rows, float* grad_weights, gunet_stream_t stream);
+
+/* Microscaled 4-bit floating point (OCP MXFP4).  A block is 32 consecutive columns of a row (the last one of a row may be
+ * shorter); its scale is 2^(floor(log2 amax) - 2), at least 2^-127, kept as exponent + 127 in a byte (0 where
+ * amax = 0); an element is x / scale rounded to nearest even on 0, .5, 1, 1.5, 2, 3, 4, 6 and saturated at 6, kept as sign bit 3
+ * and the level's number 0..7.  A block that holds a NaN or an infinity has the byte 255: all of it reads as NaN.
+ * With blocks = ceil(k / 32), for a matrix [groups, rows, k]:
+ *   codes  uint8 [groups, rows, blocks, 16]          element c of a block: byte c / 2, low four bits for even c
+ *   scales uint8 [groups, ceil(blocks / 8), rows, 8]  the scale of block b of a row: [b / 8, row, b % 8]; the
+ *                                                    entries behind the last block must not be 255 (quantize writes 0),
+ *                                                    nor may codes behind column k be other than 0
+ * codes 16-byte, scales 8-byte aligned.  groups <= 65535, rows <= 2^31 - 1, 1 <= k <= 2^22. */
+size_t gunet_mxfp4_code_bytes(int64_t groups, int64_t rows, int32_t k);
+size_t gunet_mxfp4_scale_bytes(int64_t groups, int64_t rows, int32_t k);
+int gunet_mxfp4_quantize(const void* x, int32_t dtype, int64_t groups, int64_t rows, int32_t k, uint8_t* codes,
+                         uint8_t* scales, gunet_stream_t stream);
+int gunet_mxfp4_dequantize(const uint8_t* codes, const uint8_t* scales, int64_t groups, int64_t rows, int32_t k, void* out,
+                           int32_t dtype, gunet_stream_t stream);
+
+/* Dense on 4-bit weights: out = act(q(x) @ w^T + bias) with q(x) the quantised x [rows, k] and w [n_out, k] (one row per output
+ * column: the transpose of a Dense kernel).  Products are exact, sums float32; the bias (float32 [n_out] or NULL) is added last,
+ * then the activation, then one rounding to out_dtype.  A linear layer hands a NaN on, the ReLU of a NaN is 0
+ * as in the float32 layers.  Independent of the matmul mode.  workspace: the quantised x,
+ * gunet_mxfp4_dense_workspace_bytes(rows, k) bytes, 16-byte aligned. */
+size_t gunet_mxfp4_dense_workspace_bytes(int64_t rows, int32_t k);
+int gunet_mxfp4_dense_forward(const void* x, int32_t dtype, int64_t rows, int32_t k, const uint8_t* w_codes,
+                              const uint8_t* w_scales, const float* bias, int32_t n_out, int32_t activation, void* out,
+                              int32_t out_dtype, void* workspace, size_t workspace_bytes, gunet_stream_t stream);
+
+/* The experts' Dense layers: out[r] = act(q(row r) @ w[e]^T + bias[e]) for the rows r of expert e, zeros behind
+ * offsets[n_experts].  With slot: x [n_tokens, k], row r is the token whose choice has slot r (the dispatch happens on the 4-bit
+ * rows); slot = NULL: x [n_tokens * top_k, k] is in expert order already.  w [n_experts, n_out, k], bias float32 [n_experts, n_out]
+ * or NULL, out [n_tokens * top_k, n_out].  workspace: gunet_mxfp4_dense_workspace_bytes(n_tokens * top_k, k) bytes, 16-byte
+ * aligned. */
+int gunet_mxfp4_expert_dense_forward(const void* x, int32_t dtype, const int32_t* offsets, const int32_t* slot,
+                                     int64_t n_tokens, int32_t top_k, int32_t n_experts, int32_t k, const uint8_t* w_codes,
+                                     const uint8_t* w_scales, const float* bias, int32_t n_out, int32_t activation, void* out,
+                                     int32_t out_dtype, void* workspace, size_t workspace_bytes, gunet_stream_t stream);
+
+/* ------------------------------------------------------------------------
  * 3. Either side of the model -- graph construction, input assembly (models/base_model.py:274-312),
  *    prediction image and metric sums (asynchronous and allocation-free except gunet_image_to_graph)
  * ------------------------------------------------------------------------ */
