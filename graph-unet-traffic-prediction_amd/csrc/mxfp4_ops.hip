@@ -167,6 +167,7 @@ struct ProductArgs {
   int32_t act, out_dtype;
   int64_t row_tiles;          // upper bound, over all groups
   int32_t col_tiles;
+  int32_t out_wide;           // every row of out starts on 16 bytes
 };
 
 struct RowTile {
@@ -242,45 +243,299 @@ __device__ __forceinline__ v16f mfma_fp4(uint4 a, uint4 b, v16f c, int step, int
   }
 }
 
-// The simple form: a wave computes 32 rows x 32 columns straight from memory.  Within a K tile of 8 blocks half-wave h takes
-// blocks 4h..4h+3, one per instruction, so its four scales are one dword.
-template <bool ANY_ACT>
-__global__ __launch_bounds__(kThreads) void k_mxfp4_product(ProductArgs a) {
+// 16 bytes per lane from memory straight into LDS: lane l's land at lds_base + 16 l.  The compiler does not see the load: the caller
+// waits for it before a barrier.  What lies out of the buffer's range reads as zeros.
+__device__ __forceinline__ void dma_to_lds(u32x4 rsrc, uint32_t lds_base, uint32_t lane_off, uint32_t uniform_off) {
+  asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(lds_base), "v"(lane_off), "s"(rsrc), "s"(uniform_off)
+               : "memory", "m0");
+}
+// Waits until at most N of this wave's loads are on their way and its LDS reads are done, then for the other waves.
+template <int N>
+__device__ __forceinline__ void wait_and_barrier() {
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ u32x4 rsrc_of(const void* p, uint32_t bytes) {
+  const uint64_t at = reinterpret_cast<uint64_t>(p);
+  u32x4 r = {static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(at))),
+             static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(at >> 32) & 0xFFFF)),
+             static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(bytes))), 0x00020000u};
+  return r;
+}
+
+// LDS operations of one wave run in order; this keeps the compiler from reordering those of different lanes.
+__device__ __forceinline__ void wave_lds_fence() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); }
+
+constexpr uint32_t kOutOfRange = 0x7FFFFFF0u;   // a lane offset past every buffer here (256 rows x 512 KiB)
+
+// The tiled form: a workgroup of WM x WN waves computes BM rows x BN columns, a wave FM x FN fragments of 32 x 32.  K tiles of 256
+// columns (128 bytes a row, and 8 bytes of scales) go through STAGES LDS buffers, filled by direct loads STAGES - 1 tiles ahead of the
+// one being multiplied; one barrier per tile.  A row's eight blocks lie in LDS permuted by the row's number (block b at place
+// b ^ (row / 2 & 7)), which spreads any 16 neighbouring rows that a fragment load reads one block of over all 64 banks
+// (two rows of 128 bytes span them once).  The weights are the instruction's first operand, so that a lane ends up with four
+// neighbouring columns of one output row.
+template <int WM, int WN, int FM, int FN, int STAGES, bool ANY_ACT>
+__global__ __launch_bounds__(64 * WM * WN) void k_mxfp4_tile(ProductArgs a) {
+  constexpr int BM = WM * FM * 32, BN = WN * FN * 32, NW = WM * WN;
+  constexpr int CA = BM / 8 / NW, CB = BN / 8 / NW;                          // 8-row pieces per wave
+  constexpr int SA = (BM + 127) / 128, SB = (BN + 127) / 128;                // scale pieces of 128 rows
+  constexpr int kLoads = CA + CB + 1;                                        // loads per wave and K tile
+  constexpr uint32_t kScales = (BM + BN) * 128, kBuf = kScales + (SA + SB) * 1024;
+  static_assert(NW % 2 == 0, "a wave's 8-row pieces must all have the parity of its number");
+  static_assert(SA + SB <= NW, "one scale piece per wave");
+  static_assert((STAGES - 2) * kLoads < 64, "vmcnt counts to 63");
+  extern __shared__ __attribute__((aligned(128))) char mx_smem[];
   const int lane = threadIdx.x & 63, r = lane & 31, h = lane >> 5;
-  const int wave = threadIdx.x >> 6;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = wave / WN, wn = wave % WN;
+
+  // consecutive workgroups go to different XCDs: hand each XCD a run of tiles, walked in bands of 8 row tiles so that the tiles in
+  // flight on an XCD share their operands in its L2
+  const int64_t grid = a.row_tiles * a.col_tiles;
+  int64_t tile = blockIdx.x;
+  if (grid % 8 == 0) tile = (tile % 8) * (grid / 8) + tile / 8;
+  const int64_t band = tile / (8 * a.col_tiles), in_band = tile - band * 8 * a.col_tiles;
+  const int64_t band_rows = min(static_cast<int64_t>(8), a.row_tiles - band * 8);
   RowTile t;
-  if (!find_row_tile(a, 32, blockIdx.x / a.col_tiles, &t)) return;
-  const int col0 = static_cast<int>(blockIdx.x % a.col_tiles) * 128 + wave * 32;
-  if (col0 >= a.n_out) return;
-  const int col = col0 + r;
+  if (!find_row_tile(a, BM, band * 8 + in_band % band_rows, &t)) return;
+  const int col0 = static_cast<int>(in_band / band_rows) * BN;
+  const int cols = min(BN, a.n_out - col0);
   if (t.group == a.groups) {
-    if (col < a.n_out)
-      for (int i = h; i < t.rows; i += 2) store_out(a.out, a.out_dtype, (t.row0 + i) * a.n_out + col, 0.0f);
+    for (int i = threadIdx.x; i < t.rows * BN; i += 64 * NW)
+      if (i % BN < cols) store_out(a.out, a.out_dtype, (t.row0 + i / BN) * a.n_out + col0 + i % BN, 0.0f);
     return;
   }
-  const bool row_ok = r < t.rows, col_ok = col < a.n_out;
-  const uint4* xc = reinterpret_cast<const uint4*>(a.x_codes) + (t.row0 + r) * a.blocks;
-  const uint4* wc = reinterpret_cast<const uint4*>(a.w_codes) + (static_cast<int64_t>(t.group) * a.n_out + col) * a.blocks;
-  v16f acc = {};
+
+  const uint32_t stride = static_cast<uint32_t>(a.blocks) * 16;
+  const int64_t w_row0 = static_cast<int64_t>(t.group) * a.n_out + col0;
+  const u32x4 x_rsrc = rsrc_of(a.x_codes + t.row0 * stride, static_cast<uint32_t>(t.rows) * stride);
+  const u32x4 w_rsrc = rsrc_of(a.w_codes + w_row0 * stride, static_cast<uint32_t>(cols) * stride);
+  const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)mx_smem));
+  const int my_block = (lane & 7) ^ (((wave & 1) << 2) + (lane >> 4));   // place ^ (row / 2 & 7)
+  const uint32_t lane_off = static_cast<uint32_t>(wave * 8 + (lane >> 3)) * stride + my_block * 16;
+  // the wave's scale piece (waves beyond SA + SB repeat one: every wave has the same number of loads on its way)
+  const int piece = wave % (SA + SB);
+  const bool x_piece = piece < SA;
+  const uint8_t* const scales = x_piece ? a.x_scales + t.row0 * 8 : a.w_scales + (static_cast<int64_t>(t.group) * a.tiles * a.n_out + col0) * 8;
+  const int64_t scale_step = (x_piece ? a.rows : static_cast<int64_t>(a.n_out)) * 8;
+  const uint32_t scale_bytes = static_cast<uint32_t>(x_piece ? t.rows : cols) * 8;
+  const uint32_t scale_off = static_cast<uint32_t>(x_piece ? piece : piece - SA) * 1024 + lane * 16;
+
+  auto fetch = [&](int kt, int buf) {
+    const uint32_t base = lds0 + buf * kBuf + wave * 1024;
+    const bool tail = (kt + 1) * kTileBlocks > a.blocks;       // the last tile of a row that ends inside it
+    const bool none = tail && kt * kTileBlocks + my_block >= a.blocks;
+    const uint32_t step = 8 * NW * stride;
+#pragma unroll
+    for (int i = 0; i < CA; ++i) dma_to_lds(x_rsrc, base + i * NW * 1024, none ? kOutOfRange : lane_off + i * step, kt * 128);
+#pragma unroll
+    for (int i = 0; i < CB; ++i) dma_to_lds(w_rsrc, base + BM * 128 + i * NW * 1024, none ? kOutOfRange : lane_off + i * step, kt * 128);
+    dma_to_lds(rsrc_of(scales + kt * scale_step, scale_bytes), lds0 + buf * kBuf + kScales + piece * 1024, scale_off, 0);
+  };
+
+  v16f acc[FN][FM];
+#pragma unroll
+  for (int n = 0; n < FN; ++n)
+#pragma unroll
+    for (int m = 0; m < FM; ++m) acc[n][m] = v16f{};
+
+#pragma unroll
+  for (int s = 0; s < STAGES - 1; ++s)
+    if (s < a.tiles) fetch(s, s);
+  int buf = 0;
   for (int kt = 0; kt < a.tiles; ++kt) {
-    int xs = 0, ws = 0;
-    if (row_ok) xs = reinterpret_cast<const int*>(a.x_scales)[(static_cast<int64_t>(kt) * a.rows + t.row0 + r) * 2 + h];
-    if (col_ok) ws = reinterpret_cast<const int*>(a.w_scales)[((static_cast<int64_t>(t.group) * a.tiles + kt) * a.n_out + col) * 2 + h];
+    if (kt + STAGES - 2 < a.tiles)
+      wait_and_barrier<(STAGES - 2) * kLoads>();
+    else
+      wait_and_barrier<0>();
+    if (kt + STAGES - 1 < a.tiles) fetch(kt + STAGES - 1, buf == 0 ? STAGES - 1 : buf - 1);
+    const char* const base = mx_smem + buf * kBuf;
+    int xs[FM], ws[FN];
+#pragma unroll
+    for (int f = 0; f < FM; ++f) xs[f] = *reinterpret_cast<const int*>(base + kScales + ((wm * FM + f) * 32 + r) * 8 + h * 4);
+#pragma unroll
+    for (int f = 0; f < FN; ++f) ws[f] = *reinterpret_cast<const int*>(base + kScales + SA * 1024 + ((wn * FN + f) * 32 + r) * 8 + h * 4);
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
-      const int b = kt * kTileBlocks + 4 * h + s;
-      uint4 xv = {}, wv = {};
-      if (row_ok && b < a.blocks) xv = xc[b];
-      if (col_ok && b < a.blocks) wv = wc[b];
-      acc = mfma_fp4(xv, wv, acc, s, xs, ws);
+      const int place = ((4 * h + s) ^ (r >> 1 & 7)) * 16;
+      uint4 xf[FM], wf[FN];
+#pragma unroll
+      for (int f = 0; f < FM; ++f) xf[f] = *reinterpret_cast<const uint4*>(base + ((wm * FM + f) * 32 + r) * 128 + place);
+#pragma unroll
+      for (int f = 0; f < FN; ++f) wf[f] = *reinterpret_cast<const uint4*>(base + (BM + (wn * FN + f) * 32 + r) * 128 + place);
+#pragma unroll
+      for (int n = 0; n < FN; ++n)
+#pragma unroll
+        for (int m = 0; m < FM; ++m) acc[n][m] = mfma_fp4(wf[n], xf[m], acc[n][m], s, ws[n], xs[m]);
+    }
+    buf = buf == STAGES - 1 ? 0 : buf + 1;
+  }
+
+  // Lane (r, h) holds row r of a fragment, columns 8 j + 4 h + 0..3 in acc[4 j .. 4 j + 3]: stored from there a wave's 8-byte pieces would
+  // touch 32 rows per instruction.  They go through LDS (the K tiles' space, a region per wave) 32 rows at a time and leave
+  // as whole rows of the wave's columns, 16 bytes a lane (8192^3: 0.12 ms less than stores from the fragments).
+  wait_and_barrier<0>();
+  constexpr int kStage = 32 * (FN * 128 + 16) + FN * 128;     // per wave: 32 rows of its columns in 32 bits, and its bias
+  static_assert(NW * kStage <= STAGES * kBuf, "the output's way out needs more LDS than the K tiles");
+  char* const stage = mx_smem + wave * kStage;
+  float* const bias = reinterpret_cast<float*>(stage + 32 * (FN * 128 + 16));
+  const int wave_col = wn * FN * 32, wave_cols = min(FN * 32, cols - wave_col);
+  if (wave_cols <= 0) return;
+  if (lane < FN * 32) bias[lane] = a.bias && lane < wave_cols ? a.bias[w_row0 + wave_col + lane] : 0.0f;
+  static_assert(FN <= 2, "one lane per column of the wave");
+  wave_lds_fence();
+  const int64_t at = (t.row0 + wm * FM * 32) * a.n_out + col0 + wave_col;
+
+  // fragment row m of the wave -> LDS in type T (an extra 16 bytes per row turn the rows against the banks)
+  const auto to_stage = [&](auto tag, int m, bool activate) __attribute__((always_inline)) {
+    using T = typename decltype(tag)::type;
+    constexpr int kRow = FN * 32 * sizeof(T) + 16;
+#pragma unroll
+    for (int n = 0; n < FN; ++n)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float4 b = lds_load_f4(bias + n * 32 + 8 * j + 4 * h);
+        Pack<T, 4> v;
+        const float sum[4] = {acc[n][m][4 * j] + b.x, acc[n][m][4 * j + 1] + b.y, acc[n][m][4 * j + 2] + b.z, acc[n][m][4 * j + 3] + b.w};
+#pragma unroll
+        for (int c = 0; c < 4; ++c) v.v[c] = from_f32<T>(activate && a.act == GUNET_ACT_RELU ? fmaxf(sum[c], 0.0f) : sum[c]);
+        store_pack<T, 4>(reinterpret_cast<T*>(stage + r * kRow) + n * 32 + 8 * j + 4 * h, v);
+      }
+    wave_lds_fence();
+  };
+  const auto wide = [&](auto tag) __attribute__((always_inline)) {
+    using T = typename decltype(tag)::type;
+    constexpr int kPer = 16 / sizeof(T), kRow = FN * 32 * sizeof(T) + 16, kLanes = FN * 32 / kPer;   // lanes per row
+#pragma unroll
+    for (int m = 0; m < FM; ++m) {
+      to_stage(tag, m, true);
+      const int rows = t.rows - (wm * FM + m) * 32;
+      T* const out = static_cast<T*>(a.out) + at + static_cast<int64_t>(m) * 32 * a.n_out;
+#pragma unroll
+      for (int i = 0; i < 32 * kLanes / 64; ++i) {
+        const int row = (i * 64 + lane) / kLanes, col = lane % kLanes * kPer;
+        const float4 v = lds_load_f4(reinterpret_cast<const float*>(stage + row * kRow + col * sizeof(T)));
+        if (row < rows && col < wave_cols) *reinterpret_cast<float4*>(out + static_cast<int64_t>(row) * a.n_out + col) = v;
+      }
+      wave_lds_fence();
+    }
+  };
+  if (!ANY_ACT && a.out_wide) {
+    if (a.out_dtype == GUNET_DTYPE_F32)
+      wide(TypeTag<float, 4>{});
+    else if (a.out_dtype == GUNET_DTYPE_BF16)
+      wide(TypeTag<__bf16, 8>{});
+    else
+      wide(TypeTag<_Float16, 8>{});
+    return;
+  }
+  // rows that do not start on 16 bytes, and the activations with code of their own: element by element, still along the rows
+#pragma unroll
+  for (int m = 0; m < FM; ++m) {
+    to_stage(TypeTag<float, 4>{}, m, false);
+    const int rows = min(32, t.rows - (wm * FM + m) * 32);
+#pragma nounroll
+    for (int i = lane; i < rows * FN * 32; i += 64) {
+      const int row = i / (FN * 32), col = i % (FN * 32);
+      const float v = *(reinterpret_cast<const volatile float*>(stage + row * (FN * 128 + 16)) + col);
+      if (col < wave_cols) store_out(a.out, a.out_dtype, at + static_cast<int64_t>(m * 32 + row) * a.n_out + col, finish<ANY_ACT>(v, 0.0f, a.act));
+    }
+    wave_lds_fence();
+  }
+}
+
+
+typedef float v4f __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ v4f mfma16_fp4(u32x4 a, u32x4 b, v4f c, int step, int a_scale, int b_scale) {
+  const v8i av = {static_cast<int>(a[0]), static_cast<int>(a[1]), static_cast<int>(a[2]), static_cast<int>(a[3]), 0, 0, 0, 0};
+  const v8i bv = {static_cast<int>(b[0]), static_cast<int>(b[1]), static_cast<int>(b[2]), static_cast<int>(b[3]), 0, 0, 0, 0};
+  switch (step) {
+    case 0: return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(av, bv, c, 4, 4, 0, a_scale, 0, b_scale);
+    case 1: return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(av, bv, c, 4, 4, 1, a_scale, 1, b_scale);
+    case 2: return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(av, bv, c, 4, 4, 2, a_scale, 2, b_scale);
+    default: return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(av, bv, c, 4, 4, 3, a_scale, 3, b_scale);
+  }
+}
+
+// The form for few rows, where the time is the weights' bytes: a workgroup computes 16 columns for up to 16 * MF rows, its NW waves
+// share the K axis out among them in turns of 512 columns (v_mfma_scale_f32_16x16x128: quarter-wave q takes blocks 4 q + s of 16, s = 0..3, its
+// scales again one dword), straight from memory to registers with the next turn's loads on their way, and add their parts through LDS in
+// wave order.  No barrier inside the K loop.
+template <int MF, int NW, bool ANY_ACT>
+__global__ __launch_bounds__(64 * NW) void k_mxfp4_skinny(ProductArgs a) {
+  __shared__ __attribute__((aligned(16))) float parts[NW][MF][16][16 + 4];    // [wave][row fragment][row][column]
+  const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  RowTile t;
+  if (!find_row_tile(a, 16 * MF, blockIdx.x / a.col_tiles, &t)) return;
+  const int col0 = static_cast<int>(blockIdx.x % a.col_tiles) * 16;
+  const int cols = min(16, a.n_out - col0);
+  v4f acc[MF];
+#pragma unroll
+  for (int m = 0; m < MF; ++m) acc[m] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+  if (t.group < a.groups) {
+    const uint32_t stride = static_cast<uint32_t>(a.blocks) * 16;
+    const int64_t w_row0 = static_cast<int64_t>(t.group) * a.n_out + col0;
+    const BufferRsrc xr = buffer_of(a.x_codes + t.row0 * stride, static_cast<uint32_t>(t.rows) * stride);
+    const BufferRsrc wr = buffer_of(a.w_codes + w_row0 * stride, static_cast<uint32_t>(cols) * stride);
+    const uint8_t* const xs_base = a.x_scales + t.row0 * 8;
+    const uint8_t* const ws_base = a.w_scales + (static_cast<int64_t>(t.group) * a.tiles * a.n_out + col0) * 8;
+    const int turns = (a.blocks + 15) / 16;
+    struct Turn {
+      u32x4 w[4], x[MF][4];
+      int ws, xs[MF];
+    };
+    const auto fetch = [&](int turn, Turn& f) __attribute__((always_inline)) {
+      // 256 columns per group of scales: quarter-waves 0, 1 read the turn's first group, 2, 3 its second, which a short row may not have
+      const bool second = 2 * turn + 1 < a.tiles;
+      const int64_t kt = 2 * turn + (q >> 1);
+      const bool have = second || q < 2;
+      f.ws = have && r < cols ? *reinterpret_cast<const int*>(ws_base + (kt * a.n_out + r) * 8 + (q & 1) * 4) : 0;
+#pragma unroll
+      for (int m = 0; m < MF; ++m)
+        f.xs[m] = have && m * 16 + r < t.rows ? *reinterpret_cast<const int*>(xs_base + (kt * a.rows + m * 16 + r) * 8 + (q & 1) * 4) : 0;
+#pragma unroll
+      for (int s = 0; s < 4; ++s) {
+        const int block = turn * 16 + 4 * q + s;
+        f.w[s] = __builtin_amdgcn_raw_buffer_load_b128(wr, block < a.blocks ? r * stride + block * 16 : kOutOfRange, 0, 0);
+#pragma unroll
+        for (int m = 0; m < MF; ++m)
+          f.x[m][s] = __builtin_amdgcn_raw_buffer_load_b128(xr, block < a.blocks ? (m * 16 + r) * stride + block * 16 : kOutOfRange, 0, 0);
+      }
+    };
+    const auto multiply = [&](const Turn& f) __attribute__((always_inline)) {
+#pragma unroll
+      for (int s = 0; s < 4; ++s)
+#pragma unroll
+        for (int m = 0; m < MF; ++m) acc[m] = mfma16_fp4(f.w[s], f.x[m][s], acc[m], s, f.ws, f.xs[m]);
+    };
+    Turn even, odd;
+    int turn = wave;
+    if (turn < turns) fetch(turn, even);
+    while (turn < turns) {
+      if (turn + NW < turns) fetch(turn + NW, odd);
+      multiply(even);
+      turn += NW;
+      if (turn >= turns) break;
+      if (turn + NW < turns) fetch(turn + NW, even);
+      multiply(odd);
+      turn += NW;
     }
   }
-  if (!col_ok) return;
-  const float bias = a.bias ? a.bias[static_cast<int64_t>(t.group) * a.n_out + col] : 0.0f;
+  // lane (r, q) holds row r of the fragment, columns 4 q .. 4 q + 3
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const int row = (i & 3) + 8 * (i >> 2) + 4 * h;
-    if (row < t.rows) store_out(a.out, a.out_dtype, (t.row0 + row) * a.n_out + col, finish<ANY_ACT>(acc[i], bias, a.act));
+  for (int m = 0; m < MF; ++m) *reinterpret_cast<v4f*>(&parts[wave][m][r][4 * q]) = acc[m];
+  __syncthreads();
+  for (int i = threadIdx.x; i < MF * 256; i += 64 * NW) {
+    const int m = i >> 8, row = (i >> 4) & 15, col = i & 15;
+    if (m * 16 + row >= t.rows || col >= cols) continue;
+    float v = 0.0f;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) v += parts[w][m][row][col];
+    if (t.group < a.groups) {
+      const float b = a.bias ? a.bias[static_cast<int64_t>(t.group) * a.n_out + col0 + col] : 0.0f;
+      v = finish<ANY_ACT>(v, b, a.act);
+    }
+    store_out(a.out, a.out_dtype, (t.row0 + m * 16 + row) * a.n_out + col0 + col, v);
   }
 }
 
@@ -327,19 +582,61 @@ int launch_quantize(const void* x, int32_t dtype, int64_t groups, int64_t rows, 
   return GUNET_OK;
 }
 
-int launch_product(ProductArgs a, hipStream_t stream) {
-  constexpr int kRows = 32, kCols = 128;
-  a.row_tiles = a.offsets ? std::min<int64_t>(a.rows, a.rows / kRows + a.groups + 1) : ceil_div(a.rows, kRows);
-  a.col_tiles = static_cast<int32_t>(ceil_div(a.n_out, kCols));
+template <int WM, int WN, int FM, int FN, int STAGES>
+int launch_tile(ProductArgs a, hipStream_t stream) {
+  constexpr int BM = WM * FM * 32, BN = WN * FN * 32;
+  constexpr int kLds = STAGES * ((BM + BN) * 128 + ((BM + 127) / 128 + (BN + 127) / 128) * 1024);
+  a.row_tiles = a.offsets ? std::min<int64_t>(a.rows, a.rows / BM + a.groups + 1) : ceil_div(a.rows, BM);
+  a.col_tiles = static_cast<int32_t>(ceil_div(a.n_out, BN));
   GUNET_REQUIRE(a.row_tiles * a.col_tiles <= INT32_MAX, "mxfp4 product: %lld x %d is more than one launch holds",
                 static_cast<long long>(a.rows), a.n_out);
-  const unsigned grid = static_cast<unsigned>(a.row_tiles * a.col_tiles);
-  if (act_tuned(a.act))
-    k_mxfp4_product<false><<<grid, kThreads, 0, stream>>>(a);
-  else
-    k_mxfp4_product<true><<<grid, kThreads, 0, stream>>>(a);
+  auto* const kernel = act_tuned(a.act) ? &k_mxfp4_tile<WM, WN, FM, FN, STAGES, false> : &k_mxfp4_tile<WM, WN, FM, FN, STAGES, true>;
+  if (kLds > (64 << 10))
+    GUNET_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, kLds));
+  kernel<<<static_cast<unsigned>(a.row_tiles * a.col_tiles), 64 * WM * WN, kLds, stream>>>(a);
   GUNET_LAUNCH_CHECK();
   return GUNET_OK;
+}
+
+template <int MF, int NW>
+int launch_skinny(ProductArgs a, hipStream_t stream) {
+  constexpr int BM = 16 * MF;
+  a.row_tiles = a.offsets ? std::min<int64_t>(a.rows, a.rows / BM + a.groups + 1) : ceil_div(a.rows, BM);
+  a.col_tiles = static_cast<int32_t>(ceil_div(a.n_out, 16));
+  GUNET_REQUIRE(a.row_tiles * a.col_tiles <= INT32_MAX, "mxfp4 product: %lld x %d is more than one launch holds",
+                static_cast<long long>(a.rows), a.n_out);
+  auto* const kernel = act_tuned(a.act) ? &k_mxfp4_skinny<MF, NW, false> : &k_mxfp4_skinny<MF, NW, true>;
+  kernel<<<static_cast<unsigned>(a.row_tiles * a.col_tiles), 64 * NW, 0, stream>>>(a);
+  GUNET_LAUNCH_CHECK();
+  return GUNET_OK;
+}
+
+// Which form.  Rows per group decide how many rows a tile can fill, the number of tiles whether they fill the chip (256 CUs).
+// Measured, product alone (us):
+//   rows x k x n         16 columns a workgroup   64 x 64   128 x 128   256 x 256
+//   1 x 4096 x 4096              3.4                8.5       12.8        27.6
+//   32 x 4096 x 4096             5.6                8.6
+//   64 x 4096 x 4096             8.1                8.7       13.8        28.2
+//   256 x 4096 x 4096           24.3                9.8
+//   2048 x 8192 x 1024                             20.6       26.7        52.0
+//   1024 x 2048 x 4096                             15.9       11.9        20.9
+//   48332 x 256 x 256                              19.9       11.9        13.2
+//   4096 x 4096 x 4096                             84.5       50.6        43.1
+//   8192 x 8192 x 8192                              590        381         328
+// and for 32 experts 2048 -> 4096 (quantisation included), average rows per expert 4 / 8 / 32: 16 columns 28.5 / 35.1 / 79, 64 x 64 36.8 / 38.8 / 49.
+int launch_product(ProductArgs a, hipStream_t stream) {
+  a.out_wide = reinterpret_cast<uintptr_t>(a.out) % 16 == 0 && a.n_out * dtype_size(a.out_dtype) % 16 == 0;
+  const int64_t per_group = a.offsets ? ceil_div(a.rows, a.groups) : a.rows;
+  const auto tiles = [&](int64_t size) { return (a.rows / size + (a.offsets ? a.groups / 2 : 1)) * ceil_div(a.n_out, size); };
+  if (per_group <= (a.offsets ? 8 : 16)) {
+    // two waves a workgroup stream as well as four once there are four workgroups per CU, and leave more of them side by side (1.18x)
+    if (std::min<int64_t>(a.rows, a.rows / 16 + a.groups) * ceil_div(a.n_out, 16) >= 1024) return launch_skinny<1, 2>(a, stream);
+    return launch_skinny<1, 4>(a, stream);
+  }
+  if (a.offsets == nullptr && a.rows <= 32) return launch_skinny<2, 4>(a, stream);
+  if (per_group >= 256 && tiles(256) >= 256) return launch_tile<2, 4, 4, 2, 2>(a, stream);
+  if (per_group >= 96 && tiles(128) >= 256) return launch_tile<2, 4, 2, 1, 2>(a, stream);
+  return launch_tile<2, 2, 1, 1, 4>(a, stream);
 }
 
 int64_t align256(int64_t v) { return (v + 255) / 256 * 256; }
