@@ -226,6 +226,27 @@ def current_stream(device):
     return C.c_void_p(torch.cuda.current_stream(device).cuda_stream)
 
 
+def launch(fn_name, device, *args):
+    """call(fn_name, *args, stream) on the current stream of `device`, whichever device is current (the null stream belongs
+    to the current one).  Pointers are plain addresses: for calls whose kernels take a few microseconds."""
+    import torch
+    index = device.index
+    if torch.cuda.current_device() != index:
+        with torch.cuda.device(index):
+            return launch(fn_name, device, *args)
+    status = getattr(lib, fn_name)(*args, _raw_stream(index))
+    if status != 0:
+        raise GunetError(fn_name, status, last_error())
+
+
+def _raw_stream(index):
+    """hipStream_t of the device's current stream as an integer."""
+    global _raw_stream
+    import torch
+    _raw_stream = getattr(torch._C, '_cuda_getCurrentRawStream', None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
+    return _raw_stream(index)
+
+
 def profile_enable(on):
     call('gunet_profile_enable', 1 if on else 0)
 

@@ -13,6 +13,7 @@
 // the instruction multiplies by both blocks' scales, so the data goes from memory to the matrix core as
 // it lies; sums are float32.
 #include <algorithm>
+#include <type_traits>
 
 #include "common.h"
 #include "lowp.h"
@@ -44,9 +45,44 @@ struct QuantArgs {
   const int32_t* slot;    // [rows][top_k] rows to write, or null: row r goes to row r
 };
 
-// Four lanes share a block, eight elements each: the block's amax takes two exchanges inside a group of four lanes, the codes of
-// a lane are one dword.  HBM-bound: x is read once, 17/32 byte per element written (per choice, where rows are
-// sorted by expert: quantising on the way replaces a dispatch of the unquantised rows).
+// Eight elements of a row from column `col` on (columns past k read as 0): the lane's share of its block.
+template <typename T, bool VEC>
+__device__ __forceinline__ void load_eight(const T* row, int col, int k, float (&v)[8]) {
+  if (VEC && col + 8 <= k) {
+    constexpr int kPer = 16 / sizeof(T);
+#pragma unroll
+    for (int p = 0; p < 8 / kPer; ++p) {
+      const Pack<T, kPer> q = load_pack<T, kPer>(row + col + p * kPer);
+#pragma unroll
+      for (int c = 0; c < kPer; ++c) v[p * kPer + c] = to_f32(q.v[c]);
+    }
+  } else {
+#pragma unroll
+    for (int c = 0; c < 8; ++c) v[c] = col + c < k ? to_f32(row[col + c]) : 0.0f;
+  }
+}
+
+// Four neighbouring lanes hold a block, eight elements each: returns the lane's eight codes and the block's scale byte.
+__device__ __forceinline__ uint32_t quantize_eight(const float (&v)[8], uint32_t* byte) {
+  // magnitudes as integers: NaN sorts above infinity, infinity above every number
+  uint32_t top = 0;
+#pragma unroll
+  for (int c = 0; c < 8; ++c) top = max(top, __float_as_uint(v[c]) & 0x7FFFFFFFu);
+  top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 1)));
+  top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 2)));
+  const int exponent = static_cast<int>(top >> 23);
+  *byte = exponent == 255 ? 255u : static_cast<uint32_t>(max(exponent - 2, 0));
+  if (exponent == 255) return 0;
+  const float s = scale_value(*byte);
+  uint32_t word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0u, v[0], v[1], s, 0);
+  word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, v[2], v[3], s, 1);
+  word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, v[4], v[5], s, 2);
+  return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, v[6], v[7], s, 3);
+}
+
+// Four lanes share a block: its amax takes two exchanges inside a group of four lanes, the codes of a lane are one dword.  HBM-bound: x
+// is read once, 17/32 byte per element written (per choice, where rows are sorted by expert: quantising on the way
+// replaces a dispatch of the unquantised rows).  8192 x 8192 bf16 in 36.8 us, 4.6 TB/s.
 template <typename T, bool VEC>
 __global__ __launch_bounds__(kThreads) void k_mxfp4_quantize(QuantArgs a, const T* __restrict__ x, uint8_t* __restrict__ codes,
                                                              uint8_t* __restrict__ scales) {
@@ -60,37 +96,11 @@ __global__ __launch_bounds__(kThreads) void k_mxfp4_quantize(QuantArgs a, const 
   for (int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; i < a.rows * parts; i += static_cast<int64_t>(gridDim.x) * kThreads) {
     const int64_t row = i / parts;
     const int part = static_cast<int>(i - row * parts);
-    const int block = part >> 2, col = part * 8;
+    const int block = part >> 2;
     float v[8];
-    const T* src = x + row * a.k + col;
-    if (VEC && col + 8 <= a.k) {
-      constexpr int kPer = 16 / sizeof(T);
-#pragma unroll
-      for (int p = 0; p < 8 / kPer; ++p) {
-        const Pack<T, kPer> q = load_pack<T, kPer>(src + p * kPer);
-#pragma unroll
-        for (int c = 0; c < kPer; ++c) v[p * kPer + c] = to_f32(q.v[c]);
-      }
-    } else {
-#pragma unroll
-      for (int c = 0; c < 8; ++c) v[c] = col + c < a.k ? to_f32(src[c]) : 0.0f;
-    }
-    // magnitudes as integers: NaN sorts above infinity, infinity above every number
-    uint32_t top = 0;
-#pragma unroll
-    for (int c = 0; c < 8; ++c) top = max(top, __float_as_uint(v[c]) & 0x7FFFFFFFu);
-    top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 1)));
-    top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 2)));
-    const int exponent = static_cast<int>(top >> 23);
-    const uint32_t byte = exponent == 255 ? 255u : static_cast<uint32_t>(max(exponent - 2, 0));
-    uint32_t word = 0;
-    if (exponent != 255) {
-      const float s = scale_value(byte);
-      word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, v[0], v[1], s, 0);
-      word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, v[2], v[3], s, 1);
-      word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, v[4], v[5], s, 2);
-      word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, v[6], v[7], s, 3);
-    }
+    load_eight<T, VEC>(x + row * a.k, part * 8, a.k, v);
+    uint32_t byte;
+    const uint32_t word = quantize_eight(v, &byte);
     const int copies = a.slot ? a.top_k : 1;
     for (int j = 0; j < copies; ++j) {
       int64_t r = row;
@@ -155,6 +165,8 @@ __global__ __launch_bounds__(kThreads) void k_mxfp4_dequantize(int64_t rows, int
 
 // out[r][n] = act(sum_k x[r][k] w[g][n][k] + bias[g][n]) for the rows of group g.
 struct ProductArgs {
+  const void* x;              // [rows][k], for the form that quantises on the way
+  int32_t k;
   const uint8_t* x_codes;     // [rows][blocks * 16]
   const uint8_t* x_scales;    // [tiles][rows][8]
   const uint8_t* w_codes;     // [groups][n_out][blocks * 16]
@@ -460,9 +472,13 @@ __device__ __forceinline__ v4f mfma16_fp4(u32x4 a, u32x4 b, v4f c, int step, int
 // share the K axis out among them in turns of 512 columns (v_mfma_scale_f32_16x16x128: quarter-wave q takes blocks 4 q + s of 16, s = 0..3, its
 // scales again one dword), straight from memory to registers with the next turn's loads on their way, and add their parts through LDS in
 // wave order.  No barrier inside the K loop.
-template <int MF, int NW, bool ANY_ACT>
+// XT = void: x comes quantised.  Else x is [rows][k] of that type, and every workgroup quantises its rows into LDS while its first weights
+// are on their way, which saves the launch (and the time) of doing it before; one group, MF = 1.
+template <int MF, int NW, typename XT, bool VEC, bool ANY_ACT>
 __global__ __launch_bounds__(64 * NW) void k_mxfp4_skinny(ProductArgs a) {
+  constexpr bool kRaw = !std::is_same<XT, void>::value;
   __shared__ __attribute__((aligned(16))) float parts[NW][MF][16][16 + 4];    // [wave][row fragment][row][column]
+  extern __shared__ __attribute__((aligned(16))) char raw_smem[];              // kRaw: codes [rows][blocks][16], scales [rows][tiles][8]
   const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   RowTile t;
@@ -475,34 +491,47 @@ __global__ __launch_bounds__(64 * NW) void k_mxfp4_skinny(ProductArgs a) {
   if (t.group < a.groups) {
     const uint32_t stride = static_cast<uint32_t>(a.blocks) * 16;
     const int64_t w_row0 = static_cast<int64_t>(t.group) * a.n_out + col0;
-    const BufferRsrc xr = buffer_of(a.x_codes + t.row0 * stride, static_cast<uint32_t>(t.rows) * stride);
+    const BufferRsrc xr = buffer_of(kRaw ? nullptr : a.x_codes + t.row0 * stride, static_cast<uint32_t>(t.rows) * stride);
     const BufferRsrc wr = buffer_of(a.w_codes + w_row0 * stride, static_cast<uint32_t>(cols) * stride);
-    const uint8_t* const xs_base = a.x_scales + t.row0 * 8;
+    const uint8_t* const xs_base = kRaw ? nullptr : a.x_scales + t.row0 * 8;
     const uint8_t* const ws_base = a.w_scales + (static_cast<int64_t>(t.group) * a.tiles * a.n_out + col0) * 8;
+    char* const raw_scales = raw_smem + (kRaw ? t.rows * static_cast<int>(stride) : 0);
     const int turns = (a.blocks + 15) / 16;
     struct Turn {
       u32x4 w[4], x[MF][4];
       int ws, xs[MF];
     };
+    // 256 columns per group of scales: quarter-waves 0, 1 read the turn's first group, 2, 3 its second, which a short row may not have
     const auto fetch = [&](int turn, Turn& f) __attribute__((always_inline)) {
-      // 256 columns per group of scales: quarter-waves 0, 1 read the turn's first group, 2, 3 its second, which a short row may not have
-      const bool second = 2 * turn + 1 < a.tiles;
       const int64_t kt = 2 * turn + (q >> 1);
-      const bool have = second || q < 2;
+      const bool have = kt < a.tiles;
       f.ws = have && r < cols ? *reinterpret_cast<const int*>(ws_base + (kt * a.n_out + r) * 8 + (q & 1) * 4) : 0;
+      if constexpr (!kRaw) {
 #pragma unroll
-      for (int m = 0; m < MF; ++m)
-        f.xs[m] = have && m * 16 + r < t.rows ? *reinterpret_cast<const int*>(xs_base + (kt * a.rows + m * 16 + r) * 8 + (q & 1) * 4) : 0;
+        for (int m = 0; m < MF; ++m)
+          f.xs[m] = have && m * 16 + r < t.rows ? *reinterpret_cast<const int*>(xs_base + (kt * a.rows + m * 16 + r) * 8 + (q & 1) * 4) : 0;
+      }
 #pragma unroll
       for (int s = 0; s < 4; ++s) {
         const int block = turn * 16 + 4 * q + s;
         f.w[s] = __builtin_amdgcn_raw_buffer_load_b128(wr, block < a.blocks ? r * stride + block * 16 : kOutOfRange, 0, 0);
+        if constexpr (!kRaw) {
 #pragma unroll
-        for (int m = 0; m < MF; ++m)
-          f.x[m][s] = __builtin_amdgcn_raw_buffer_load_b128(xr, block < a.blocks ? (m * 16 + r) * stride + block * 16 : kOutOfRange, 0, 0);
+          for (int m = 0; m < MF; ++m)
+            f.x[m][s] = __builtin_amdgcn_raw_buffer_load_b128(xr, block < a.blocks ? (m * 16 + r) * stride + block * 16 : kOutOfRange, 0, 0);
+        }
       }
     };
-    const auto multiply = [&](const Turn& f) __attribute__((always_inline)) {
+    const auto multiply = [&](int turn, Turn& f) __attribute__((always_inline)) {
+      if constexpr (kRaw) {     // lanes of rows that are not there repeat the last one: their results are not stored
+        const int row = min(r, t.rows - 1), kt = 2 * turn + (q >> 1);
+        f.xs[0] = kt < a.tiles ? *reinterpret_cast<const int*>(raw_scales + (row * a.tiles + kt) * 8 + (q & 1) * 4) : 0;
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+          const int block = turn * 16 + 4 * q + s;
+          f.x[0][s] = block < a.blocks ? *reinterpret_cast<const u32x4*>(raw_smem + row * stride + block * 16) : u32x4{0, 0, 0, 0};
+        }
+      }
 #pragma unroll
       for (int s = 0; s < 4; ++s)
 #pragma unroll
@@ -511,13 +540,29 @@ __global__ __launch_bounds__(64 * NW) void k_mxfp4_skinny(ProductArgs a) {
     Turn even, odd;
     int turn = wave;
     if (turn < turns) fetch(turn, even);
+    if constexpr (kRaw) {
+      const int row_parts = a.blocks * 4;
+      for (int i = threadIdx.x; i < t.rows * row_parts; i += 64 * NW) {
+        const int row = i / row_parts, part = i - row * row_parts, block = part >> 2;
+        float v[8];
+        load_eight<XT, VEC>(static_cast<const XT*>(a.x) + (t.row0 + row) * a.k, part * 8, a.k, v);
+        uint32_t byte;
+        const uint32_t word = quantize_eight(v, &byte);
+        *reinterpret_cast<uint32_t*>(raw_smem + row * stride + part * 4) = word;
+        char* const s8 = raw_scales + row * a.tiles * 8;
+        if ((part & 3) == 0) s8[block] = static_cast<char>(byte);
+        if (part == row_parts - 1)
+          for (int b = block + 1; b < a.tiles * kTileBlocks; ++b) s8[b] = 0;
+      }
+      __syncthreads();
+    }
     while (turn < turns) {
       if (turn + NW < turns) fetch(turn + NW, odd);
-      multiply(even);
+      multiply(turn, even);
       turn += NW;
       if (turn >= turns) break;
       if (turn + NW < turns) fetch(turn + NW, even);
-      multiply(odd);
+      multiply(turn, odd);
       turn += NW;
     }
   }
@@ -598,17 +643,32 @@ int launch_tile(ProductArgs a, hipStream_t stream) {
   return GUNET_OK;
 }
 
-template <int MF, int NW>
-int launch_skinny(ProductArgs a, hipStream_t stream) {
+template <int MF, int NW, typename XT = void, bool VEC = false>
+int launch_skinny(ProductArgs a, hipStream_t stream, size_t lds = 0) {
   constexpr int BM = 16 * MF;
   a.row_tiles = a.offsets ? std::min<int64_t>(a.rows, a.rows / BM + a.groups + 1) : ceil_div(a.rows, BM);
   a.col_tiles = static_cast<int32_t>(ceil_div(a.n_out, 16));
   GUNET_REQUIRE(a.row_tiles * a.col_tiles <= INT32_MAX, "mxfp4 product: %lld x %d is more than one launch holds",
                 static_cast<long long>(a.rows), a.n_out);
-  auto* const kernel = act_tuned(a.act) ? &k_mxfp4_skinny<MF, NW, false> : &k_mxfp4_skinny<MF, NW, true>;
-  kernel<<<static_cast<unsigned>(a.row_tiles * a.col_tiles), 64 * NW, 0, stream>>>(a);
+  auto* const kernel = act_tuned(a.act) ? &k_mxfp4_skinny<MF, NW, XT, VEC, false> : &k_mxfp4_skinny<MF, NW, XT, VEC, true>;
+  kernel<<<static_cast<unsigned>(a.row_tiles * a.col_tiles), 64 * NW, lds, stream>>>(a);
   GUNET_LAUNCH_CHECK();
   return GUNET_OK;
+}
+
+// The product that quantises x on its way: LDS for the quantised rows, 0 where the form does not apply.  Every workgroup does all of it, so it
+// pays for little x only.  Whole call, one launch against two (us): 1 x 4096 x 4096 4.5 / 5.7, 1 x 8192 x 8192 9.4 / 10.3, 2 x 4096 x 4096
+// 5.4 / 6.0, 16 x 1024 x 8192 6.6 / 6.0, 4 x 4096 x 4096 7.3 / 6.2, 16 x 2048 x 2048 10.2 / 5.8.
+constexpr int64_t kRawElements = 8192;
+size_t raw_lds(const ProductArgs& a) {
+  if (a.offsets != nullptr || a.rows > 16 || a.rows * a.k > kRawElements) return 0;
+  return static_cast<size_t>(a.rows) * (a.blocks * 16 + a.tiles * 8);
+}
+
+template <typename XT>
+int launch_raw(const ProductArgs& a, size_t lds, hipStream_t stream) {
+  const bool vec = reinterpret_cast<uintptr_t>(a.x) % 16 == 0 && a.k * sizeof(XT) % 16 == 0;
+  return vec ? launch_skinny<1, 4, XT, true>(a, stream, lds) : launch_skinny<1, 4, XT, false>(a, stream, lds);
 }
 
 // Which form.  Rows per group decide how many rows a tile can fill, the number of tiles whether they fill the chip (256 CUs).
@@ -662,11 +722,9 @@ int run_dense(const char* fn, const void* x, int32_t dtype, int64_t x_rows, int6
     return GUNET_ERR_WORKSPACE;
   }
   GUNET_REQUIRE(reinterpret_cast<uintptr_t>(workspace) % 16 == 0, "%s: workspace is not 16-byte aligned", fn);
-  uint8_t* const x_codes = static_cast<uint8_t*>(workspace);
-  GUNET_TRY(launch_quantize(x, dtype, 1, x_rows, rows, k, top_k, slot, x_codes, x_codes + codes, stream));
   ProductArgs a = {};
-  a.x_codes = x_codes;
-  a.x_scales = x_codes + codes;
+  a.x = x;
+  a.k = k;
   a.w_codes = w_codes;
   a.w_scales = w_scales;
   a.bias = bias;
@@ -679,6 +737,15 @@ int run_dense(const char* fn, const void* x, int32_t dtype, int64_t x_rows, int6
   a.groups = groups;
   a.act = activation;
   a.out_dtype = out_dtype;
+  if (const size_t lds = raw_lds(a)) {
+    if (dtype == GUNET_DTYPE_F32) return launch_raw<float>(a, lds, stream);
+    if (dtype == GUNET_DTYPE_BF16) return launch_raw<__bf16>(a, lds, stream);
+    return launch_raw<_Float16>(a, lds, stream);
+  }
+  uint8_t* const x_codes = static_cast<uint8_t*>(workspace);
+  GUNET_TRY(launch_quantize(x, dtype, 1, x_rows, rows, k, top_k, slot, x_codes, x_codes + codes, stream));
+  a.x_codes = x_codes;
+  a.x_scales = x_codes + codes;
   return launch_product(a, stream);
 }
 

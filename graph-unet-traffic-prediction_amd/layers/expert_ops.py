@@ -18,7 +18,7 @@ Tensors may be strided (they are then copied first); all of them on one GPU, who
 import torch
 
 from .. import _lib
-from .._lib import call, current_stream, ptr
+from .._lib import launch
 
 DTYPES = {torch.float32: _lib.DTYPE_F32, torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_F16}
 
@@ -36,14 +36,14 @@ def checked(t, what, device=None, dtype=None, shape=None):
         raise TypeError(f'{what} must be a CUDA tensor')
     if device is not None and t.device != device:
         raise ValueError(f'{what} is on {t.device}, the other tensors are on {device}')
-    if dtype is not None and t.dtype != dtype:
+    if dtype is not None and t.dtype is not dtype:
         raise TypeError(f'{what} must be {dtype}, got {t.dtype}')
-    if shape is not None and tuple(t.shape) != tuple(shape):
+    if shape is not None and t.shape != shape:
         raise ValueError(f'{what} must have the shape {tuple(shape)}, got {tuple(t.shape)}')
     if t.requires_grad and torch.is_grad_enabled():
         raise ValueError(f'{what} requires a gradient: this call records no autograd graph (detach it, or call under '
                          'torch.no_grad() and use the _grad functions)')
-    return t.contiguous()
+    return t if t.is_contiguous() else t.contiguous()
 
 
 class ExpertPlan:
@@ -53,30 +53,27 @@ class ExpertPlan:
     def __init__(self, offsets, order, slot, n_experts):
         self.offsets, self.order, self.slot = offsets, order, slot
         self.n_experts = n_experts
-        self.n_tokens, self.top_k = slot.shape
+        self.shape = slot.shape
+        self.n_tokens, self.top_k = self.shape
+        self.n_rows = self.n_tokens * self.top_k
         self.device = slot.device
-
-    @property
-    def n_rows(self):
-        return self.n_tokens * self.top_k
 
 
 def expert_plan(expert_index, n_experts):
     """The order of the choices expert_index int32 [T, k]; a value outside 0 .. n_experts - 1 drops the choice."""
-    index = checked(expert_index, 'expert_index', dtype=torch.int32)
+    index = checked(expert_index, 'expert_index', None, torch.int32)
     if index.dim() != 2 or index.shape[1] < 1:
         raise ValueError(f'expert_index must be [T, k] with k >= 1, got {tuple(index.shape)}')
     n_experts = int(n_experts)
     t, k = index.shape
     dev = index.device
-    offsets = torch.empty(max(n_experts, 0) + 1, dtype=torch.int32, device=dev)
-    order = torch.empty(t * k, dtype=torch.int32, device=dev)
-    slot = torch.empty((t, k), dtype=torch.int32, device=dev)
+    offsets = index.new_empty(max(n_experts, 0) + 1)
+    order = index.new_empty(t * k)
+    slot = index.new_empty((t, k))
     nbytes = _lib.lib.gunet_expert_sort_workspace_bytes(t, k, n_experts)
-    scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-    with torch.cuda.device(dev):
-        call('gunet_expert_sort', ptr(index), t, k, n_experts, ptr(offsets), ptr(order), ptr(slot), ptr(scratch), nbytes,
-             current_stream(dev))
+    scratch = index.new_empty(nbytes // 4) if nbytes else None
+    launch('gunet_expert_sort', dev, index.data_ptr(), t, k, n_experts, offsets.data_ptr(), order.data_ptr(), slot.data_ptr(),
+           scratch.data_ptr() if nbytes else None, nbytes)
     return ExpertPlan(offsets, order, slot, n_experts)
 
 
@@ -90,10 +87,10 @@ def expert_dispatch(x, plan):
     """x [T, C] -> rows [T * k, C] in expert order (zeros behind the last expert's)."""
     x = checked(x, 'x', plan.device)
     width = _width(x, 'x', plan.n_tokens)
-    rows = torch.empty((plan.n_rows, width), dtype=x.dtype, device=x.device)
-    with torch.cuda.device(x.device):
-        call('gunet_expert_dispatch', ptr(x), dtype_code(x, 'x'), ptr(plan.offsets), ptr(plan.slot), plan.n_tokens, plan.top_k,
-             plan.n_experts, width, ptr(rows), current_stream(x.device))
+    code = dtype_code(x, 'x')
+    rows = x.new_empty((plan.n_rows, width))
+    launch('gunet_expert_dispatch', plan.device, x.data_ptr(), code, plan.offsets.data_ptr(), plan.slot.data_ptr(), plan.n_tokens,
+           plan.top_k, plan.n_experts, width, rows.data_ptr())
     return rows
 
 
@@ -101,10 +98,10 @@ def expert_dispatch_grad(grad_rows, plan):
     """Gradient of expert_dispatch: grad_rows [T * k, C] -> grad_x [T, C]."""
     g = checked(grad_rows, 'grad_rows', plan.device)
     width = _width(g, 'grad_rows', plan.n_rows)
-    grad_x = torch.empty((plan.n_tokens, width), dtype=g.dtype, device=g.device)
-    with torch.cuda.device(g.device):
-        call('gunet_expert_dispatch_grad', ptr(g), dtype_code(g, 'grad_rows'), ptr(plan.slot), plan.n_tokens, plan.top_k, width,
-             ptr(grad_x), current_stream(g.device))
+    code = dtype_code(g, 'grad_rows')
+    grad_x = g.new_empty((plan.n_tokens, width))
+    launch('gunet_expert_dispatch_grad', plan.device, g.data_ptr(), code, plan.slot.data_ptr(), plan.n_tokens, plan.top_k, width,
+           grad_x.data_ptr())
     return grad_x
 
 
@@ -112,11 +109,11 @@ def expert_combine(rows, weights, plan):
     """out[t] = sum_j weights[t, j] * rows[slot[t, j]]: rows [T * k, C], weights float32 [T, k] -> [T, C]."""
     rows = checked(rows, 'rows', plan.device)
     width = _width(rows, 'rows', plan.n_rows)
-    w = checked(weights, 'weights', plan.device, torch.float32, plan.slot.shape)
-    out = torch.empty((plan.n_tokens, width), dtype=rows.dtype, device=rows.device)
-    with torch.cuda.device(rows.device):
-        call('gunet_expert_combine', ptr(rows), dtype_code(rows, 'rows'), ptr(w), ptr(plan.slot), plan.n_tokens, plan.top_k, width,
-             ptr(out), current_stream(rows.device))
+    code = dtype_code(rows, 'rows')
+    w = checked(weights, 'weights', plan.device, torch.float32, plan.shape)
+    out = rows.new_empty((plan.n_tokens, width))
+    launch('gunet_expert_combine', plan.device, rows.data_ptr(), code, w.data_ptr(), plan.slot.data_ptr(), plan.n_tokens, plan.top_k,
+           width, out.data_ptr())
     return out
 
 
@@ -124,11 +121,11 @@ def expert_combine_grad(grad_out, rows, weights, plan):
     """Gradients of expert_combine: (grad_rows [T * k, C] in the type of rows, grad_weights float32 [T, k])."""
     rows = checked(rows, 'rows', plan.device)
     width = _width(rows, 'rows', plan.n_rows)
+    code = dtype_code(rows, 'rows')
     g = checked(grad_out, 'grad_out', plan.device, rows.dtype, (plan.n_tokens, width))
-    w = checked(weights, 'weights', plan.device, torch.float32, plan.slot.shape)
+    w = checked(weights, 'weights', plan.device, torch.float32, plan.shape)
     grad_rows = torch.empty_like(rows)
     grad_weights = torch.empty_like(w)
-    with torch.cuda.device(rows.device):
-        call('gunet_expert_combine_grad', ptr(g), ptr(rows), dtype_code(rows, 'rows'), ptr(w), ptr(plan.offsets), ptr(plan.slot),
-             plan.n_tokens, plan.top_k, plan.n_experts, width, ptr(grad_rows), ptr(grad_weights), current_stream(rows.device))
+    launch('gunet_expert_combine_grad', plan.device, g.data_ptr(), rows.data_ptr(), code, w.data_ptr(), plan.offsets.data_ptr(),
+           plan.slot.data_ptr(), plan.n_tokens, plan.top_k, plan.n_experts, width, grad_rows.data_ptr(), grad_weights.data_ptr())
     return grad_rows, grad_weights

@@ -11,7 +11,7 @@ gradients (a tensor that requires one is refused), nothing synchronises, everyth
 import torch
 
 from .. import _lib
-from .._lib import call, current_stream, ptr
+from .._lib import launch
 from .expert_ops import DTYPES, checked, dtype_code
 from .hybrid_gnn import _activation_code
 
@@ -64,8 +64,7 @@ def mxfp4_quantize(x):
     x = checked(x, 'x')
     code = dtype_code(x, 'x')
     t = Mxfp4Tensor.empty(x.shape, x.device)
-    with torch.cuda.device(x.device):
-        call('gunet_mxfp4_quantize', ptr(x), code, t.groups, t.rows, t.k, ptr(t.codes), ptr(t.scales), current_stream(x.device))
+    launch('gunet_mxfp4_quantize', t.device, x.data_ptr(), code, t.groups, t.rows, t.k, t.codes.data_ptr(), t.scales.data_ptr())
     return t
 
 
@@ -74,9 +73,8 @@ def mxfp4_dequantize(t, dtype=torch.float32):
     if dtype not in DTYPES:
         raise TypeError(f'dtype must be float32, bfloat16 or float16, got {dtype}')
     out = torch.empty(t.shape, dtype=dtype, device=t.device)
-    with torch.cuda.device(t.device):
-        call('gunet_mxfp4_dequantize', ptr(t.codes), ptr(t.scales), t.groups, t.rows, t.k, ptr(out), DTYPES[dtype],
-             current_stream(t.device))
+    launch('gunet_mxfp4_dequantize', t.device, t.codes.data_ptr(), t.scales.data_ptr(), t.groups, t.rows, t.k, out.data_ptr(),
+           DTYPES[dtype])
     return out
 
 
@@ -101,11 +99,11 @@ def mxfp4_dense(x, w, bias=None, activation=None, out_dtype=None):
     if len(w.shape) != 2:
         raise ValueError(f'w must be [n_out, k], got {w.shape} (mxfp4_expert_dense takes stacks)')
     rows = x.numel() // w.k
-    out = torch.empty(x.shape[:-1] + (w.rows,), dtype=out_dtype, device=x.device)
-    scratch = torch.empty(_lib.lib.gunet_mxfp4_dense_workspace_bytes(rows, w.k), dtype=torch.uint8, device=x.device)
-    with torch.cuda.device(x.device):
-        call('gunet_mxfp4_dense_forward', ptr(x), code, rows, w.k, ptr(w.codes), ptr(w.scales), ptr(bias), w.rows, act, ptr(out),
-             DTYPES[out_dtype], ptr(scratch), scratch.numel(), current_stream(x.device))
+    out = x.new_empty(x.shape[:-1] + (w.rows,), dtype=out_dtype)
+    nbytes = _lib.lib.gunet_mxfp4_dense_workspace_bytes(rows, w.k)
+    scratch = w.codes.new_empty(nbytes)
+    launch('gunet_mxfp4_dense_forward', w.device, x.data_ptr(), code, rows, w.k, w.codes.data_ptr(), w.scales.data_ptr(),
+           bias.data_ptr() if bias is not None else None, w.rows, act, out.data_ptr(), DTYPES[out_dtype], scratch.data_ptr(), nbytes)
     return out
 
 
@@ -121,12 +119,13 @@ def mxfp4_expert_dense(x, w, plan, bias=None, activation=None, out_dtype=None, s
     want = plan.n_rows if sorted_rows else plan.n_tokens
     if x.dim() != 2 or x.shape[0] != want:
         raise ValueError(f'x must be [{want}, {w.k}], got {tuple(x.shape)}')
-    out = torch.empty((plan.n_rows, w.rows), dtype=out_dtype, device=x.device)
-    scratch = torch.empty(_lib.lib.gunet_mxfp4_dense_workspace_bytes(plan.n_rows, w.k), dtype=torch.uint8, device=x.device)
-    with torch.cuda.device(x.device):
-        call('gunet_mxfp4_expert_dense_forward', ptr(x), code, ptr(plan.offsets), None if sorted_rows else ptr(plan.slot),
-             plan.n_tokens, plan.top_k, plan.n_experts, w.k, ptr(w.codes), ptr(w.scales), ptr(bias), w.rows, act, ptr(out),
-             DTYPES[out_dtype], ptr(scratch), scratch.numel(), current_stream(x.device))
+    out = x.new_empty((plan.n_rows, w.rows), dtype=out_dtype)
+    nbytes = _lib.lib.gunet_mxfp4_dense_workspace_bytes(plan.n_rows, w.k)
+    scratch = w.codes.new_empty(nbytes)
+    launch('gunet_mxfp4_expert_dense_forward', w.device, x.data_ptr(), code, plan.offsets.data_ptr(),
+           None if sorted_rows else plan.slot.data_ptr(), plan.n_tokens, plan.top_k, plan.n_experts, w.k, w.codes.data_ptr(),
+           w.scales.data_ptr(), bias.data_ptr() if bias is not None else None, w.rows, act, out.data_ptr(), DTYPES[out_dtype],
+           scratch.data_ptr(), nbytes)
     return out
 
 
