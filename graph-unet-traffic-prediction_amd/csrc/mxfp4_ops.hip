@@ -177,7 +177,6 @@ struct ProductArgs {
   int64_t rows;
   int32_t n_out, blocks, tiles, groups;
   int32_t act, out_dtype;
-  int64_t row_tiles;          // upper bound, over all groups
   int32_t col_tiles;
   int32_t out_wide;           // every row of out starts on 16 bytes
 };
@@ -188,8 +187,31 @@ struct RowTile {
   int rows;
 };
 
-// Row tile number `tile` of the groups' rows cut into tiles of at most `size` rows: every wave finds it by itself, 64 groups at a
-// time.  Offsets are taken into 0..rows, so no value of theirs leads out of a tensor.
+// First and last row of group g (g == groups: the rows behind the last group).  Offsets are taken into 0..rows, so no value of theirs leads
+// out of a tensor.
+__device__ __forceinline__ void group_rows(const ProductArgs& a, int g, int* begin, int* end) {
+  *begin = *end = 0;
+  if (g > a.groups) return;
+  const int rows = static_cast<int>(a.rows);
+  *begin = min(max(a.offsets[g], 0), rows);
+  *end = g < a.groups ? min(max(a.offsets[g + 1], 0), rows) : rows;
+}
+
+// Number of row tiles of at most `size` rows that the groups' rows are cut into.
+__device__ __forceinline__ int count_row_tiles(const ProductArgs& a, int size) {
+  if (a.offsets == nullptr) return static_cast<int>((a.rows + size - 1) / size);
+  int mine = 0;
+  for (int g = threadIdx.x & 63; g <= a.groups; g += 64) {
+    int begin, end;
+    group_rows(a, g, &begin, &end);
+    if (end > begin) mine += (end - begin + size - 1) / size;
+  }
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) mine += __shfl_xor(mine, d);
+  return __builtin_amdgcn_readfirstlane(mine);
+}
+
+// Row tile number `tile`: every wave finds it by itself, 64 groups at a time.
 __device__ __forceinline__ bool find_row_tile(const ProductArgs& a, int size, int64_t tile, RowTile* out) {
   if (a.offsets == nullptr) {
     out->group = 0;
@@ -200,13 +222,8 @@ __device__ __forceinline__ bool find_row_tile(const ProductArgs& a, int size, in
   const int lane = threadIdx.x & 63;
   int done = 0;
   for (int first = 0; first <= a.groups; first += 64) {
-    const int g = first + lane;
-    int begin = 0, end = 0;
-    if (g <= a.groups) {
-      const int rows = static_cast<int>(a.rows);
-      begin = min(max(a.offsets[g], 0), rows);
-      end = g < a.groups ? min(max(a.offsets[g + 1], 0), rows) : rows;
-    }
+    int begin, end;
+    group_rows(a, first + lane, &begin, &end);
     const int tiles = end > begin ? (end - begin + size - 1) / size : 0;
     int upto = tiles;
 #pragma unroll
@@ -274,9 +291,19 @@ __device__ __forceinline__ u32x4 rsrc_of(const void* p, uint32_t bytes) {
   return r;
 }
 
-// LDS operations of one wave run in order; this keeps the compiler from reordering those of different lanes.
-__device__ __forceinline__ void wave_lds_fence() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); }
+// LDS by its byte address.  Volatile, so that the compiler keeps the order of what different lanes of a wave write and read (the hardware does) and
+// neither merges nor cuts the accesses; through LDS's own address space, since a volatile access through a plain pointer becomes a
+// flat one, which waits for the wave's stores to memory as well.
+template <typename V>
+__device__ __forceinline__ V lds_read(uint32_t at) {
+  return *(const volatile __attribute__((address_space(3))) V*)(at);
+}
+template <typename V>
+__device__ __forceinline__ void lds_write(uint32_t at, V v) {
+  *(volatile __attribute__((address_space(3))) V*)(at) = v;
+}
 
+constexpr int kBand = 4;
 constexpr uint32_t kOutOfRange = 0x7FFFFFF0u;   // a lane offset past every buffer here (256 rows x 512 KiB)
 
 // The tiled form: a workgroup of WM x WN waves computes BM rows x BN columns, a wave FM x FN fragments of 32 x 32.  K tiles of 256
@@ -285,30 +312,51 @@ constexpr uint32_t kOutOfRange = 0x7FFFFFF0u;   // a lane offset past every buff
 // b ^ (row / 2 & 7)), which spreads any 16 neighbouring rows that a fragment load reads one block of over all 64 banks
 // (two rows of 128 bytes span them once).  The weights are the instruction's first operand, so that a lane ends up with four
 // neighbouring columns of one output row.
+template <int WM, int WN, int FM, int FN, int STAGES>
+struct TileShape {
+  static constexpr int BM = WM * FM * 32, BN = WN * FN * 32, NW = WM * WN;
+  static constexpr int SA = (BM + 127) / 128, SB = (BN + 127) / 128;          // scale pieces of 128 rows
+  static constexpr int kScales = (BM + BN) * 128, kBuf = kScales + (SA + SB) * 1024;
+  // On the way out a wave has its share of one buffer: one or two pieces of 32 rows of 128 bytes at most, and the bias of its columns.
+  static constexpr int kOutBytes = kBuf / NW / 16 * 16, kPiece = 32 * 128, kPieces = (kOutBytes - FN * 128) / kPiece >= 2 ? 2 : 1;
+  static_assert(kOutBytes >= kPiece + FN * 128, "no room for the way out");
+  static constexpr int kLds = STAGES * kBuf, kPerCu = (160 << 10) / kLds;    // workgroups per CU
+};
+
 template <int WM, int WN, int FM, int FN, int STAGES, bool ANY_ACT>
-__global__ __launch_bounds__(64 * WM * WN) void k_mxfp4_tile(ProductArgs a) {
-  constexpr int BM = WM * FM * 32, BN = WN * FN * 32, NW = WM * WN;
+__global__ __launch_bounds__(64 * WM * WN, (TileShape<WM, WN, FM, FN, STAGES>::kPerCu * WM * WN / 4)) void k_mxfp4_tile(ProductArgs a) {
+  using S = TileShape<WM, WN, FM, FN, STAGES>;
+  constexpr int BM = S::BM, BN = S::BN, NW = S::NW, SA = S::SA, SB = S::SB;
   constexpr int CA = BM / 8 / NW, CB = BN / 8 / NW;                          // 8-row pieces per wave
-  constexpr int SA = (BM + 127) / 128, SB = (BN + 127) / 128;                // scale pieces of 128 rows
   constexpr int kLoads = CA + CB + 1;                                        // loads per wave and K tile
-  constexpr uint32_t kScales = (BM + BN) * 128, kBuf = kScales + (SA + SB) * 1024;
+  constexpr uint32_t kScales = S::kScales, kBuf = S::kBuf;
   static_assert(NW % 2 == 0, "a wave's 8-row pieces must all have the parity of its number");
   static_assert(SA + SB <= NW, "one scale piece per wave");
   static_assert((STAGES - 2) * kLoads < 64, "vmcnt counts to 63");
+  static_assert(FN <= 2, "one lane per column of the wave's bias");
   extern __shared__ __attribute__((aligned(128))) char mx_smem[];
   const int lane = threadIdx.x & 63, r = lane & 31, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave / WN, wn = wave % WN;
+  const uint32_t stride = static_cast<uint32_t>(a.blocks) * 16;
+  const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)mx_smem));
+  const int my_block = (lane & 7) ^ (((wave & 1) << 2) + (lane >> 4));   // place ^ (row / 2 & 7)
+  const uint32_t lane_off = static_cast<uint32_t>(wave * 8 + (lane >> 3)) * stride + my_block * 16;
+  // the wave's scale piece (waves beyond SA + SB repeat one: every wave has the same number of loads on its way)
+  const int piece = wave % (SA + SB);
+  const bool x_piece = piece < SA;
+  const uint32_t scale_off = static_cast<uint32_t>(x_piece ? piece : piece - SA) * 1024 + lane * 16;
+  const int64_t scale_step = (x_piece ? a.rows : static_cast<int64_t>(a.n_out)) * 8;
 
-  // consecutive workgroups go to different XCDs: hand each XCD a run of tiles, walked in bands of 8 row tiles so that the tiles in
-  // flight on an XCD share their operands in its L2
-  const int64_t grid = a.row_tiles * a.col_tiles;
-  int64_t tile = blockIdx.x;
-  if (grid % 8 == 0) tile = (tile % 8) * (grid / 8) + tile / 8;
-  const int64_t band = tile / (8 * a.col_tiles), in_band = tile - band * 8 * a.col_tiles;
-  const int64_t band_rows = min(static_cast<int64_t>(8), a.row_tiles - band * 8);
+  // Consecutive workgroups go to different XCDs: each XCD gets a run of tiles, walked in bands of 4 row tiles, so that the tiles in
+  // flight on an XCD share their operands in its L2.
+  const int64_t row_tiles = count_row_tiles(a, BM), all = row_tiles * a.col_tiles, run = (all + 7) / 8;
+  const int64_t tile = (blockIdx.x & 7) * run + (blockIdx.x >> 3);
+  if ((blockIdx.x >> 3) >= run || tile >= all) return;
+  const int64_t band = tile / (kBand * a.col_tiles), in_band = tile - band * kBand * a.col_tiles;
+  const int64_t band_rows = min(static_cast<int64_t>(kBand), row_tiles - band * kBand);
   RowTile t;
-  if (!find_row_tile(a, BM, band * 8 + in_band % band_rows, &t)) return;
+  if (!find_row_tile(a, BM, band * kBand + in_band % band_rows, &t)) return;
   const int col0 = static_cast<int>(in_band / band_rows) * BN;
   const int cols = min(BN, a.n_out - col0);
   if (t.group == a.groups) {
@@ -316,23 +364,11 @@ __global__ __launch_bounds__(64 * WM * WN) void k_mxfp4_tile(ProductArgs a) {
       if (i % BN < cols) store_out(a.out, a.out_dtype, (t.row0 + i / BN) * a.n_out + col0 + i % BN, 0.0f);
     return;
   }
-
-  const uint32_t stride = static_cast<uint32_t>(a.blocks) * 16;
   const int64_t w_row0 = static_cast<int64_t>(t.group) * a.n_out + col0;
   const u32x4 x_rsrc = rsrc_of(a.x_codes + t.row0 * stride, static_cast<uint32_t>(t.rows) * stride);
   const u32x4 w_rsrc = rsrc_of(a.w_codes + w_row0 * stride, static_cast<uint32_t>(cols) * stride);
-  const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)mx_smem));
-  const int my_block = (lane & 7) ^ (((wave & 1) << 2) + (lane >> 4));   // place ^ (row / 2 & 7)
-  const uint32_t lane_off = static_cast<uint32_t>(wave * 8 + (lane >> 3)) * stride + my_block * 16;
-  // the wave's scale piece (waves beyond SA + SB repeat one: every wave has the same number of loads on its way)
-  const int piece = wave % (SA + SB);
-  const bool x_piece = piece < SA;
   const uint8_t* const scales = x_piece ? a.x_scales + t.row0 * 8 : a.w_scales + (static_cast<int64_t>(t.group) * a.tiles * a.n_out + col0) * 8;
-  const int64_t scale_step = (x_piece ? a.rows : static_cast<int64_t>(a.n_out)) * 8;
-  const uint32_t scale_bytes = static_cast<uint32_t>(x_piece ? t.rows : cols) * 8;
-  const uint32_t scale_off = static_cast<uint32_t>(x_piece ? piece : piece - SA) * 1024 + lane * 16;
-
-  auto fetch = [&](int kt, int buf) {
+  const auto fetch = [&](int kt, int buf) __attribute__((always_inline)) {
     const uint32_t base = lds0 + buf * kBuf + wave * 1024;
     const bool tail = (kt + 1) * kTileBlocks > a.blocks;       // the last tile of a row that ends inside it
     const bool none = tail && kt * kTileBlocks + my_block >= a.blocks;
@@ -341,7 +377,8 @@ __global__ __launch_bounds__(64 * WM * WN) void k_mxfp4_tile(ProductArgs a) {
     for (int i = 0; i < CA; ++i) dma_to_lds(x_rsrc, base + i * NW * 1024, none ? kOutOfRange : lane_off + i * step, kt * 128);
 #pragma unroll
     for (int i = 0; i < CB; ++i) dma_to_lds(w_rsrc, base + BM * 128 + i * NW * 1024, none ? kOutOfRange : lane_off + i * step, kt * 128);
-    dma_to_lds(rsrc_of(scales + kt * scale_step, scale_bytes), lds0 + buf * kBuf + kScales + piece * 1024, scale_off, 0);
+    dma_to_lds(rsrc_of(scales + kt * scale_step, static_cast<uint32_t>(x_piece ? t.rows : cols) * 8), lds0 + buf * kBuf + kScales + piece * 1024,
+               scale_off, 0);
   };
 
   v16f acc[FN][FM];
@@ -349,7 +386,6 @@ __global__ __launch_bounds__(64 * WM * WN) void k_mxfp4_tile(ProductArgs a) {
   for (int n = 0; n < FN; ++n)
 #pragma unroll
     for (int m = 0; m < FM; ++m) acc[n][m] = v16f{};
-
 #pragma unroll
   for (int s = 0; s < STAGES - 1; ++s)
     if (s < a.tiles) fetch(s, s);
@@ -381,55 +417,56 @@ __global__ __launch_bounds__(64 * WM * WN) void k_mxfp4_tile(ProductArgs a) {
     }
     buf = buf == STAGES - 1 ? 0 : buf + 1;
   }
+  wait_and_barrier<0>();       // every wave has read its last K tile: LDS is free
 
   // Lane (r, h) holds row r of a fragment, columns 8 j + 4 h + 0..3 in acc[4 j .. 4 j + 3]: stored from there a wave's 8-byte pieces would
-  // touch 32 rows per instruction.  They go through LDS (the K tiles' space, a region per wave) 32 rows at a time and leave
-  // as whole rows of the wave's columns, 16 bytes a lane (8192^3: 0.12 ms less than stores from the fragments).
-  wait_and_barrier<0>();
-  constexpr int kStage = 32 * (FN * 128 + 16) + FN * 128;     // per wave: 32 rows of its columns in 32 bits, and its bias
-  static_assert(NW * kStage <= STAGES * kBuf, "the output's way out needs more LDS than the K tiles");
-  char* const stage = mx_smem + wave * kStage;
-  float* const bias = reinterpret_cast<float*>(stage + 32 * (FN * 128 + 16));
+  // touch 32 rows per instruction.  They go through LDS (a region per wave) in pieces of 32 rows x 128 bytes, 16-byte chunks permuted by the
+  // row against the banks, and leave 16 bytes a lane as whole lines (8192^3: 0.12 ms less than stores from the fragments), past the caches, which have the operands to hold (16 experts, 268 MB of results: 237 us against 248).
+  const uint32_t stage = lds0 + wave * S::kOutBytes, bias_at = stage + S::kPieces * S::kPiece;
   const int wave_col = wn * FN * 32, wave_cols = min(FN * 32, cols - wave_col);
-  if (wave_cols <= 0) return;
-  if (lane < FN * 32) bias[lane] = a.bias && lane < wave_cols ? a.bias[w_row0 + wave_col + lane] : 0.0f;
-  static_assert(FN <= 2, "one lane per column of the wave");
-  wave_lds_fence();
-  const int64_t at = (t.row0 + wm * FM * 32) * a.n_out + col0 + wave_col;
+  if (lane < FN * 32) lds_write(bias_at + lane * 4, a.bias && lane < wave_cols ? a.bias[w_row0 + wave_col + lane] : 0.0f);
+  const int64_t out0 = (t.row0 + wm * FM * 32) * a.n_out + col0 + wave_col;
 
-  // fragment row m of the wave -> LDS in type T (an extra 16 bytes per row turn the rows against the banks)
-  const auto to_stage = [&](auto tag, int m, bool activate) __attribute__((always_inline)) {
+  // Fragment row m from column fragment n0 on, in type T: to LDS in 32 rows of kRow bytes, and out through emit(LDS address, kRow, chunk mask)
+  const auto piece_out = [&](auto tag, int m, int n0, int which, bool activate, auto emit) __attribute__((always_inline)) {
     using T = typename decltype(tag)::type;
-    constexpr int kRow = FN * 32 * sizeof(T) + 16;
+    constexpr int P = sizeof(T) == 4 ? 1 : FN, kRow = P * 32 * sizeof(T), kTurn = kRow / 16 - 1;
+    const uint32_t base = stage + which * S::kPiece;
 #pragma unroll
-    for (int n = 0; n < FN; ++n)
+    for (int n = 0; n < P; ++n)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const float4 b = lds_load_f4(bias + n * 32 + 8 * j + 4 * h);
-        Pack<T, 4> v;
-        const float sum[4] = {acc[n][m][4 * j] + b.x, acc[n][m][4 * j + 1] + b.y, acc[n][m][4 * j + 2] + b.z, acc[n][m][4 * j + 3] + b.w};
+        typedef T Four __attribute__((ext_vector_type(4)));
+        const f32x4n b = lds_read<f32x4n>(bias_at + ((n0 + n) * 32 + 8 * j + 4 * h) * 4);
+        Four v;
 #pragma unroll
-        for (int c = 0; c < 4; ++c) v.v[c] = from_f32<T>(activate && a.act == GUNET_ACT_RELU ? fmaxf(sum[c], 0.0f) : sum[c]);
-        store_pack<T, 4>(reinterpret_cast<T*>(stage + r * kRow) + n * 32 + 8 * j + 4 * h, v);
+        for (int c = 0; c < 4; ++c) {
+          const float sum = acc[n0 + n][m][4 * j + c] + b[c];
+          v[c] = from_f32<T>(activate && a.act == GUNET_ACT_RELU ? fmaxf(sum, 0.0f) : sum);
+        }
+        const int byte = (n * 32 + 8 * j + 4 * h) * sizeof(T);
+        lds_write(base + r * kRow + ((byte >> 4 ^ (r * kRow / 128 & kTurn)) << 4) + (byte & 15), v);
       }
-    wave_lds_fence();
+    emit(base, kRow, kTurn);
   };
   const auto wide = [&](auto tag) __attribute__((always_inline)) {
     using T = typename decltype(tag)::type;
-    constexpr int kPer = 16 / sizeof(T), kRow = FN * 32 * sizeof(T) + 16, kLanes = FN * 32 / kPer;   // lanes per row
+    constexpr int P = sizeof(T) == 4 ? 1 : FN;
 #pragma unroll
-    for (int m = 0; m < FM; ++m) {
-      to_stage(tag, m, true);
-      const int rows = t.rows - (wm * FM + m) * 32;
-      T* const out = static_cast<T*>(a.out) + at + static_cast<int64_t>(m) * 32 * a.n_out;
+    for (int m = 0; m < FM; ++m)
 #pragma unroll
-      for (int i = 0; i < 32 * kLanes / 64; ++i) {
-        const int row = (i * 64 + lane) / kLanes, col = lane % kLanes * kPer;
-        const float4 v = lds_load_f4(reinterpret_cast<const float*>(stage + row * kRow + col * sizeof(T)));
-        if (row < rows && col < wave_cols) *reinterpret_cast<float4*>(out + static_cast<int64_t>(row) * a.n_out + col) = v;
-      }
-      wave_lds_fence();
-    }
+      for (int n = 0; n < FN; n += P)
+        piece_out(tag, m, n, (m * FN + n) / P % S::kPieces, true, [&](uint32_t base, int row_bytes, int turn) __attribute__((always_inline)) {
+          const int lanes = row_bytes / 16, rows = t.rows - (wm * FM + m) * 32;
+          const int chunk = lane % lanes, col = n * 32 + chunk * (16 / sizeof(T));
+          T* const out = static_cast<T*>(a.out) + out0 + static_cast<int64_t>(m) * 32 * a.n_out + col;
+#pragma unroll
+          for (int i = 0; i < lanes / 2; ++i) {
+            const int row = (i * 64 + lane) / lanes;
+            const u32x4 v = lds_read<u32x4>(base + row * row_bytes + ((chunk ^ (row * row_bytes / 128 & turn)) << 4));
+            if (row < rows && col < wave_cols) __builtin_nontemporal_store(v, reinterpret_cast<u32x4*>(out + static_cast<int64_t>(row) * a.n_out));
+          }
+        });
   };
   if (!ANY_ACT && a.out_wide) {
     if (a.out_dtype == GUNET_DTYPE_F32)
@@ -438,23 +475,24 @@ __global__ __launch_bounds__(64 * WM * WN) void k_mxfp4_tile(ProductArgs a) {
       wide(TypeTag<__bf16, 8>{});
     else
       wide(TypeTag<_Float16, 8>{});
-    return;
-  }
-  // rows that do not start on 16 bytes, and the activations with code of their own: element by element, still along the rows
+  } else {
+    // rows that do not start on 16 bytes, and the activations with code of their own: element by element, still along the rows
 #pragma unroll
-  for (int m = 0; m < FM; ++m) {
-    to_stage(TypeTag<float, 4>{}, m, false);
-    const int rows = min(32, t.rows - (wm * FM + m) * 32);
+    for (int m = 0; m < FM; ++m)
+#pragma unroll
+      for (int n = 0; n < FN; ++n)
+        piece_out(TypeTag<float, 4>{}, m, n, 0, false, [&](uint32_t base, int row_bytes, int turn) __attribute__((always_inline)) {
+          const int rows = min(32, t.rows - (wm * FM + m) * 32);
 #pragma nounroll
-    for (int i = lane; i < rows * FN * 32; i += 64) {
-      const int row = i / (FN * 32), col = i % (FN * 32);
-      const float v = *(reinterpret_cast<const volatile float*>(stage + row * (FN * 128 + 16)) + col);
-      if (col < wave_cols) store_out(a.out, a.out_dtype, at + static_cast<int64_t>(m * 32 + row) * a.n_out + col, finish<ANY_ACT>(v, 0.0f, a.act));
-    }
-    wave_lds_fence();
+          for (int i = lane; i < rows * 32; i += 64) {
+            const int row = i / 32, col = i % 32;
+            const float v = lds_read<float>(base + row * row_bytes + ((col >> 2 ^ (row & turn)) << 4) + (col & 3) * 4);
+            const int c = n * 32 + col;
+            if (c < wave_cols) store_out(a.out, a.out_dtype, out0 + static_cast<int64_t>(m * 32 + row) * a.n_out + c, finish<ANY_ACT>(v, 0.0f, a.act));
+          }
+        });
   }
 }
-
 
 typedef float v4f __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ v4f mfma16_fp4(u32x4 a, u32x4 b, v4f c, int step, int a_scale, int b_scale) {
@@ -629,16 +667,15 @@ int launch_quantize(const void* x, int32_t dtype, int64_t groups, int64_t rows, 
 
 template <int WM, int WN, int FM, int FN, int STAGES>
 int launch_tile(ProductArgs a, hipStream_t stream) {
-  constexpr int BM = WM * FM * 32, BN = WN * FN * 32;
-  constexpr int kLds = STAGES * ((BM + BN) * 128 + ((BM + 127) / 128 + (BN + 127) / 128) * 1024);
-  a.row_tiles = a.offsets ? std::min<int64_t>(a.rows, a.rows / BM + a.groups + 1) : ceil_div(a.rows, BM);
-  a.col_tiles = static_cast<int32_t>(ceil_div(a.n_out, BN));
-  GUNET_REQUIRE(a.row_tiles * a.col_tiles <= INT32_MAX, "mxfp4 product: %lld x %d is more than one launch holds",
-                static_cast<long long>(a.rows), a.n_out);
+  using S = TileShape<WM, WN, FM, FN, STAGES>;
+  const int64_t row_tiles = a.offsets ? std::min<int64_t>(a.rows, a.rows / S::BM + a.groups + 1) : ceil_div(a.rows, S::BM);
+  a.col_tiles = static_cast<int32_t>(ceil_div(a.n_out, S::BN));
   auto* const kernel = act_tuned(a.act) ? &k_mxfp4_tile<WM, WN, FM, FN, STAGES, false> : &k_mxfp4_tile<WM, WN, FM, FN, STAGES, true>;
-  if (kLds > (64 << 10))
-    GUNET_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, kLds));
-  kernel<<<static_cast<unsigned>(a.row_tiles * a.col_tiles), 64 * WM * WN, kLds, stream>>>(a);
+  if (S::kLds > (64 << 10))
+    GUNET_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, S::kLds));
+  const int64_t grid = ceil_div(row_tiles * a.col_tiles, 8) * 8;
+  GUNET_REQUIRE(grid <= INT32_MAX, "mxfp4 product: %lld x %d is more than one launch holds", static_cast<long long>(a.rows), a.n_out);
+  kernel<<<static_cast<unsigned>(grid), 64 * S::NW, S::kLds, stream>>>(a);
   GUNET_LAUNCH_CHECK();
   return GUNET_OK;
 }
@@ -646,12 +683,12 @@ int launch_tile(ProductArgs a, hipStream_t stream) {
 template <int MF, int NW, typename XT = void, bool VEC = false>
 int launch_skinny(ProductArgs a, hipStream_t stream, size_t lds = 0) {
   constexpr int BM = 16 * MF;
-  a.row_tiles = a.offsets ? std::min<int64_t>(a.rows, a.rows / BM + a.groups + 1) : ceil_div(a.rows, BM);
+  const int64_t row_tiles = a.offsets ? std::min<int64_t>(a.rows, a.rows / BM + a.groups + 1) : ceil_div(a.rows, BM);
   a.col_tiles = static_cast<int32_t>(ceil_div(a.n_out, 16));
-  GUNET_REQUIRE(a.row_tiles * a.col_tiles <= INT32_MAX, "mxfp4 product: %lld x %d is more than one launch holds",
+  GUNET_REQUIRE(row_tiles * a.col_tiles <= INT32_MAX, "mxfp4 product: %lld x %d is more than one launch holds",
                 static_cast<long long>(a.rows), a.n_out);
   auto* const kernel = act_tuned(a.act) ? &k_mxfp4_skinny<MF, NW, XT, VEC, false> : &k_mxfp4_skinny<MF, NW, XT, VEC, true>;
-  kernel<<<static_cast<unsigned>(a.row_tiles * a.col_tiles), 64 * NW, lds, stream>>>(a);
+  kernel<<<static_cast<unsigned>(row_tiles * a.col_tiles), 64 * NW, lds, stream>>>(a);
   GUNET_LAUNCH_CHECK();
   return GUNET_OK;
 }
