@@ -394,7 +394,7 @@ int check_shape(const char* fn, int64_t n_tokens, int32_t top_k, int32_t n_exper
 int check_rows(const char* fn, int32_t dtype, int64_t n_tokens, int32_t top_k, int32_t n_experts, int64_t width) {
   GUNET_TRY(check_shape(fn, n_tokens, top_k, n_experts));
   GUNET_REQUIRE(dtype_valid(dtype), "%s: dtype %d is none of GUNET_DTYPE_*", fn, dtype);
-  GUNET_REQUIRE(width >= 0 && width <= INT32_MAX, "%s: width %lld", fn, static_cast<long long>(width));
+  GUNET_REQUIRE(width >= 0 && width <= (1 << 30), "%s: width %lld (0..2^30)", fn, static_cast<long long>(width));
   return GUNET_OK;
 }
 

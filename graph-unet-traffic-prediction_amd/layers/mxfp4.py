@@ -23,18 +23,30 @@ class Mxfp4Tensor:
     [groups, ceil(blocks / 8), rows, 8], the layout of include/gunet_hip.h."""
 
     def __init__(self, codes, scales, shape):
-        self.codes, self.scales, self.shape = codes, scales, tuple(shape)
+        self.shape = tuple(shape)
+        want = self._layout(self.shape)
+        for t, what, size in ((codes, 'codes', want[0]), (scales, 'scales', want[1])):
+            if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dtype is torch.uint8):
+                raise TypeError(f'{what} must be a uint8 CUDA tensor')
+            if t.shape != size or not t.is_contiguous() or t.data_ptr() % 16 or t.device != codes.device:
+                raise ValueError(f'{what} must be packed {size} on 16 bytes, on one device, got {tuple(t.shape)} on {t.device}')
+        self.codes, self.scales = codes, scales
         self.groups, self.rows, self.k = ((1,) + self.shape)[-3:]
         self.device = codes.device
 
-    @classmethod
-    def empty(cls, shape, device):
+    @staticmethod
+    def _layout(shape):
         if len(shape) not in (2, 3) or shape[-1] < 1:
             raise ValueError(f'a 4-bit tensor is [rows, k] or [groups, rows, k] with k >= 1, got {tuple(shape)}')
         groups, rows, k = ((1,) + tuple(shape))[-3:]
         blocks = -(-k // BLOCK)
-        return cls(torch.empty((groups, rows, blocks, 16), dtype=torch.uint8, device=device),
-                   torch.empty((groups, -(-blocks // 8), rows, 8), dtype=torch.uint8, device=device), shape)
+        return (groups, rows, blocks, 16), (groups, -(-blocks // 8), rows, 8)
+
+    @classmethod
+    def empty(cls, shape, device):
+        """Room for a tensor of that shape, contents undefined."""
+        codes, scales = cls._layout(shape)
+        return cls(torch.empty(codes, dtype=torch.uint8, device=device), torch.empty(scales, dtype=torch.uint8, device=device), shape)
 
     @classmethod
     def from_codes(cls, codes, scales, k):

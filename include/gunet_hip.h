@@ -394,7 +394,7 @@ int gunet_expert_sort(const int32_t* expert_index, int64_t n_tokens, int32_t top
                       int32_t* order, int32_t* slot, void* workspace, size_t workspace_bytes, gunet_stream_t stream);
 
 /* rows[slot[t][j]] = x[t] for every kept choice, zeros in the rows behind offsets[n_experts]: x [n_tokens, width],
- * rows [n_tokens * top_k, width], both of type `dtype`.  Outputs may not overlap inputs (here and below). */
+ * rows [n_tokens * top_k, width], both of type `dtype`, 0 <= width <= 2^30.  Outputs may not overlap inputs (here and below). */
 int gunet_expert_dispatch(const void* x, int32_t dtype, const int32_t* offsets, const int32_t* slot, int64_t n_tokens,
                           int32_t top_k, int32_t n_experts, int64_t width, void* rows, gunet_stream_t stream);
 /* Its gradient: grad_x[t] = sum_j grad_rows[slot[t][j]], float32 sums from j = 0 up, rounded once. */
@@ -429,10 +429,11 @@ int gunet_mxfp4_dequantize(const uint8_t* codes, const uint8_t* scales, int64_t 
                            int32_t dtype, gunet_stream_t stream);
 
 /* Dense on 4-bit weights: out = act(q(x) @ w^T + bias) with q(x) the quantised x [rows, k] and w [n_out, k] (one row per output
- * column: the transpose of a Dense kernel).  Products are exact, sums float32; the bias (float32 [n_out] or NULL) is added last,
+ * column: the transpose of a Dense kernel), n_out >= 1.  Products are exact (below 2^-126 they may be 0), sums float32; the bias (float32 [n_out] or NULL) is added last,
  * then the activation, then one rounding to out_dtype.  A linear layer hands a NaN on, the ReLU of a NaN is 0
- * as in the float32 layers.  Independent of the matmul mode.  workspace: the quantised x,
- * gunet_mxfp4_dense_workspace_bytes(rows, k) bytes, 16-byte aligned. */
+ * as in the float32 layers.  Independent of the matmul mode.  The order of the sums depends on the sizes, not on the run.
+ * workspace: the quantised x, gunet_mxfp4_dense_workspace_bytes(rows, k) bytes, 16-byte aligned; calls that may overlap in
+ * time need one each. */
 size_t gunet_mxfp4_dense_workspace_bytes(int64_t rows, int32_t k);
 int gunet_mxfp4_dense_forward(const void* x, int32_t dtype, int64_t rows, int32_t k, const uint8_t* w_codes,
                               const uint8_t* w_scales, const float* bias, int32_t n_out, int32_t activation, void* out,

@@ -44,7 +44,7 @@ def test_rows(lib):
         return lib.gunet_expert_combine_grad(g, rows, dtype, w, offsets, slot, t, k, e, width, gr, gw, None)
 
     for fn in (dispatch, dispatch_grad, combine, grad):
-        for kw in (dict(dtype=3), dict(dtype=-1), dict(t=-1), dict(k=0), dict(t=2 ** 31), dict(width=-1), dict(width=2 ** 31), dict(slot=None)):
+        for kw in (dict(dtype=3), dict(dtype=-1), dict(t=-1), dict(k=0), dict(t=2 ** 31), dict(width=-1), dict(width=2 ** 30 + 1), dict(slot=None)):
             assert fn(**kw) == INVALID, (fn.__name__, kw)
         assert fn(t=0) == OK
     for fn in (dispatch, dispatch_grad, combine):

@@ -152,6 +152,53 @@ def test_dense_against_the_exact_product(amd, dtype, rows, k, n):
     assert torch.equal(got, amd.mxfp4_dense(x, w4, torch.as_tensor(bias).cuda(), 'relu', torch.float32))
 
 
+@pytest.mark.parametrize('dtype, rows, k, n', [
+    (torch.float32, 3001, 300, 2001), (torch.bfloat16, 3000, 33, 2056), (torch.float16, 5003, 96, 1028),         # 128 x 128 tiles
+    (torch.float32, 4999, 520, 4104), (torch.bfloat16, 4353, 288, 4099), (torch.float16, 4999, 32, 4112),        # 256 x 256 tiles
+    (torch.bfloat16, 300, 100, 16384), (torch.float32, 20, 1000, 20000), (torch.bfloat16, 9, 2080, 16400)], ids=str)
+def test_dense_in_every_tile_size(amd, dtype, rows, k, n):
+    """Sizes that reach the large tiles, with ragged edges on both sides, and few rows with many columns."""
+    rng = np.random.default_rng(rows)
+    x, w4 = _features(rng, (rows, k), dtype), amd.mxfp4_quantize(_features(rng, (n, k), torch.float32))
+    bias = torch.as_tensor(rng.standard_normal(n), dtype=torch.float32).cuda()
+    x64, w64 = _plain(amd.mxfp4_quantize(x)), _plain(w4)
+    _check_product(amd.mxfp4_dense(x, w4, bias, 'relu'), x64, w64, bias.double().cpu().numpy(), True, dtype)
+    _check_product(amd.mxfp4_dense(x, w4, None, None, torch.float32), x64, w64, None, False, torch.float32)
+
+
+def test_generic_activation_in_large_tiles(amd, oracle):
+    rng = np.random.default_rng(8)
+    w = amd.mxfp4_quantize(_features(rng, (4104, 64), torch.float32) * 0.05)
+    for rows in (1500, 4500):
+        x = _features(rng, (rows, 64), torch.float32)
+        before = amd.mxfp4_dense(x, w).double().cpu().numpy()
+        got = amd.mxfp4_dense(x, w, None, 'tanh').double().cpu().numpy()
+        assert np.abs(got - np.tanh(before)).max() <= 1e-5
+
+
+@pytest.mark.parametrize('t, top_k, e, k, n', [(3000, 2, 3, 160, 3000), (1700, 1, 6, 40, 8200), (700, 3, 40, 64, 4104)])
+def test_expert_dense_in_every_tile_size(amd, t, top_k, e, k, n):
+    """Uneven experts, one of them empty and one of a single row, in tiles of 256, 128 and 64 rows."""
+    rng = np.random.default_rng(t)
+    index = rng.integers(-1, e, (t, top_k)).astype(np.int32)
+    index[index == 1] = 0
+    index[5, 0] = 1
+    if e > 4:
+        index[index == 4] = 2
+    plan = amd.expert_plan(torch.as_tensor(index).cuda(), e)
+    x = _features(rng, (t, k), torch.bfloat16)
+    w4 = amd.mxfp4_quantize(_features(rng, (e, n, k), torch.bfloat16))
+    bias = torch.as_tensor(rng.standard_normal((e, n)), dtype=torch.float32).cuda()
+    q = R.dispatch(_plain(amd.mxfp4_quantize(x)), plan.slot.cpu().numpy())
+    offsets = plan.offsets.cpu().numpy()
+    got = amd.mxfp4_expert_dense(x, w4, plan, bias)
+    w64 = _plain3(w4)
+    for i in range(e):
+        a, b = offsets[i], offsets[i + 1]
+        _check_product(got[a:b], q[a:b], w64[i], bias[i].double().cpu().numpy(), False, torch.bfloat16)
+    assert not got[offsets[-1]:].any() and offsets[-1] < t * top_k
+
+
 @pytest.mark.parametrize('rows', [3, 40, 300])
 def test_every_activation(amd, oracle, rows):
     """Both sides evaluate the activation of the same float32 sum, so only the function's own error counts: the float32 gate of the
@@ -359,3 +406,8 @@ def test_refusals(amd):
         amd.Mxfp4Tensor.from_codes(torch.zeros((8, 30), dtype=torch.uint8).cuda(), torch.zeros((8, 2), dtype=torch.uint8).cuda(), 64)
     with pytest.raises(ValueError):
         amd.Mxfp4Dense.from_dense(amd.hybrid_gnn.Dense(8))
+    for codes, scales in ((w.codes[:, :7], w.scales), (w.codes, w.scales[:, :, :7]), (w.codes.transpose(1, 2), w.scales)):
+        with pytest.raises(ValueError):
+            amd.Mxfp4Tensor(codes, scales, (8, 64))
+    with pytest.raises(TypeError):
+        amd.Mxfp4Tensor(w.codes.int(), w.scales, (8, 64))
