@@ -7,6 +7,8 @@ is used by the callers for device memory and streams only.
 import ctypes as C
 import os
 
+import torch
+
 _HERE = os.path.dirname(os.path.abspath(__file__))
 # GUNET_HIP_LIBRARY: another build of the same library (A/B timing of kernel variants)
 LIB_PATH = os.environ.get('GUNET_HIP_LIBRARY') or os.path.join(_HERE, 'libgunet_hip.so')
@@ -170,6 +172,7 @@ SIGNATURES = {
     'gunet_mxfp4_dense_forward': (C.c_int, [C.c_void_p, C.c_int32, C.c_int64, C.c_int32, C.c_void_p, C.c_void_p,
                                             C.c_void_p, C.c_int32, C.c_int32, C.c_void_p, C.c_int32, C.c_void_p,
                                             C.c_size_t, C.c_void_p]),
+    'gunet_mxfp4_expert_dense_workspace_bytes': (C.c_size_t, [C.c_int64, C.c_int32]),
     'gunet_mxfp4_expert_dense_forward': (C.c_int, [C.c_void_p, C.c_int32, C.c_void_p, C.c_void_p, C.c_int64, C.c_int32,
                                                    C.c_int32, C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int32,
                                                    C.c_int32, C.c_void_p, C.c_int32, C.c_void_p, C.c_size_t,
@@ -222,29 +225,25 @@ def ptr4(tensors):
 
 
 def current_stream(device):
-    import torch
     return C.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+
+
+# hipStream_t of a device's current stream as an integer, by device index
+_raw_stream = (getattr(torch._C, '_cuda_getCurrentRawStream', None)
+               or (lambda index: torch.cuda.current_stream(index).cuda_stream))
 
 
 def launch(fn_name, device, *args):
     """call(fn_name, *args, stream) on the current stream of `device`, whichever device is current (the null stream belongs
     to the current one).  Pointers are plain addresses: for calls whose kernels take a few microseconds."""
-    import torch
     index = device.index
-    if torch.cuda.current_device() != index:
+    if torch.cuda.current_device() == index:
+        status = getattr(lib, fn_name)(*args, _raw_stream(index))
+    else:
         with torch.cuda.device(index):
-            return launch(fn_name, device, *args)
-    status = getattr(lib, fn_name)(*args, _raw_stream(index))
+            status = getattr(lib, fn_name)(*args, _raw_stream(index))
     if status != 0:
         raise GunetError(fn_name, status, last_error())
-
-
-def _raw_stream(index):
-    """hipStream_t of the device's current stream as an integer."""
-    global _raw_stream
-    import torch
-    _raw_stream = getattr(torch._C, '_cuda_getCurrentRawStream', None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
-    return _raw_stream(index)
 
 
 def profile_enable(on):

@@ -693,17 +693,15 @@ int launch_skinny(ProductArgs a, hipStream_t stream, size_t lds = 0) {
   return GUNET_OK;
 }
 
-// The product that quantises x on its way: LDS for the quantised rows, 0 where the form does not apply.  Every workgroup does all of it, so it
+// Whether the product of one group quantises x on its way.  Every workgroup does all of it, so it
 // pays for little x only.  Whole call, one launch against two (us): 1 x 4096 x 4096 4.5 / 5.7, 1 x 8192 x 8192 9.4 / 10.3, 2 x 4096 x 4096
 // 5.4 / 6.0, 16 x 1024 x 8192 6.6 / 6.0, 4 x 4096 x 4096 7.3 / 6.2, 16 x 2048 x 2048 10.2 / 5.8.
 constexpr int64_t kRawElements = 8192;
-size_t raw_lds(const ProductArgs& a) {
-  if (a.offsets != nullptr || a.rows > 16 || a.rows * a.k > kRawElements) return 0;
-  return static_cast<size_t>(a.rows) * (a.blocks * 16 + a.tiles * 8);
-}
+bool raw_form(int64_t rows, int64_t k) { return rows <= 16 && rows * k <= kRawElements; }
 
 template <typename XT>
-int launch_raw(const ProductArgs& a, size_t lds, hipStream_t stream) {
+int launch_raw(const ProductArgs& a, hipStream_t stream) {
+  const size_t lds = static_cast<size_t>(a.rows) * (a.blocks * 16 + a.tiles * 8);
   const bool vec = reinterpret_cast<uintptr_t>(a.x) % 16 == 0 && a.k * sizeof(XT) % 16 == 0;
   return vec ? launch_skinny<1, 4, XT, true>(a, stream, lds) : launch_skinny<1, 4, XT, false>(a, stream, lds);
 }
@@ -753,12 +751,6 @@ int run_dense(const char* fn, const void* x, int32_t dtype, int64_t x_rows, int6
                 "%s: codes must lie on 16 bytes, scales on 8", fn);
   GUNET_REQUIRE(reinterpret_cast<uintptr_t>(x) % dtype_size(dtype) == 0 && reinterpret_cast<uintptr_t>(out) % dtype_size(out_dtype) == 0,
                 "%s: x or out is not aligned to its type", fn);
-  const int64_t codes = align256(code_bytes(rows, k)), need = codes + scale_bytes(rows, k);
-  if (workspace == nullptr || workspace_bytes < static_cast<size_t>(need)) {
-    set_error("%s: workspace of %zu bytes, %lld are needed", fn, workspace ? workspace_bytes : size_t{0}, static_cast<long long>(need));
-    return GUNET_ERR_WORKSPACE;
-  }
-  GUNET_REQUIRE(reinterpret_cast<uintptr_t>(workspace) % 16 == 0, "%s: workspace is not 16-byte aligned", fn);
   ProductArgs a = {};
   a.x = x;
   a.k = k;
@@ -774,11 +766,17 @@ int run_dense(const char* fn, const void* x, int32_t dtype, int64_t x_rows, int6
   a.groups = groups;
   a.act = activation;
   a.out_dtype = out_dtype;
-  if (const size_t lds = raw_lds(a)) {
-    if (dtype == GUNET_DTYPE_F32) return launch_raw<float>(a, lds, stream);
-    if (dtype == GUNET_DTYPE_BF16) return launch_raw<__bf16>(a, lds, stream);
-    return launch_raw<_Float16>(a, lds, stream);
+  if (offsets == nullptr && raw_form(rows, k)) {
+    if (dtype == GUNET_DTYPE_F32) return launch_raw<float>(a, stream);
+    if (dtype == GUNET_DTYPE_BF16) return launch_raw<__bf16>(a, stream);
+    return launch_raw<_Float16>(a, stream);
   }
+  const int64_t codes = align256(code_bytes(rows, k)), need = codes + scale_bytes(rows, k);
+  if (workspace == nullptr || workspace_bytes < static_cast<size_t>(need)) {
+    set_error("%s: workspace of %zu bytes, %lld are needed", fn, workspace ? workspace_bytes : size_t{0}, static_cast<long long>(need));
+    return GUNET_ERR_WORKSPACE;
+  }
+  GUNET_REQUIRE(reinterpret_cast<uintptr_t>(workspace) % 16 == 0, "%s: workspace is not 16-byte aligned", fn);
   uint8_t* const x_codes = static_cast<uint8_t*>(workspace);
   GUNET_TRY(launch_quantize(x, dtype, 1, x_rows, rows, k, top_k, slot, x_codes, x_codes + codes, stream));
   a.x_codes = x_codes;
@@ -840,7 +838,12 @@ int gunet_mxfp4_dequantize(const uint8_t* codes, const uint8_t* scales, int64_t 
 }
 
 size_t gunet_mxfp4_dense_workspace_bytes(int64_t rows, int32_t k) {
-  if (check_matrix("mxfp4_dense_workspace_bytes", 1, rows, k) != GUNET_OK) return 0;
+  if (check_matrix("mxfp4_dense_workspace_bytes", 1, rows, k) != GUNET_OK || raw_form(rows, k)) return 0;
+  return static_cast<size_t>(align256(code_bytes(rows, k)) + scale_bytes(rows, k));
+}
+
+size_t gunet_mxfp4_expert_dense_workspace_bytes(int64_t rows, int32_t k) {
+  if (check_matrix("mxfp4_expert_dense_workspace_bytes", 1, rows, k) != GUNET_OK) return 0;
   return static_cast<size_t>(align256(code_bytes(rows, k)) + scale_bytes(rows, k));
 }
 

@@ -46,7 +46,13 @@ class Mxfp4Tensor:
     def empty(cls, shape, device):
         """Room for a tensor of that shape, contents undefined."""
         codes, scales = cls._layout(shape)
-        return cls(torch.empty(codes, dtype=torch.uint8, device=device), torch.empty(scales, dtype=torch.uint8, device=device), shape)
+        t = cls.__new__(cls)                    # what __init__ checks holds by construction
+        t.codes = torch.empty(codes, dtype=torch.uint8, device=device)
+        t.scales = t.codes.new_empty(scales)
+        t.shape = tuple(shape)
+        t.groups, t.rows, t.k = codes[0], codes[1], t.shape[-1]
+        t.device = t.codes.device
+        return t
 
     @classmethod
     def from_codes(cls, codes, scales, k):
@@ -113,9 +119,10 @@ def mxfp4_dense(x, w, bias=None, activation=None, out_dtype=None):
     rows = x.numel() // w.k
     out = x.new_empty(x.shape[:-1] + (w.rows,), dtype=out_dtype)
     nbytes = _lib.lib.gunet_mxfp4_dense_workspace_bytes(rows, w.k)
-    scratch = w.codes.new_empty(nbytes)
+    scratch = w.codes.new_empty(nbytes) if nbytes else None
     launch('gunet_mxfp4_dense_forward', w.device, x.data_ptr(), code, rows, w.k, w.codes.data_ptr(), w.scales.data_ptr(),
-           bias.data_ptr() if bias is not None else None, w.rows, act, out.data_ptr(), DTYPES[out_dtype], scratch.data_ptr(), nbytes)
+           bias.data_ptr() if bias is not None else None, w.rows, act, out.data_ptr(), DTYPES[out_dtype],
+           scratch.data_ptr() if nbytes else None, nbytes)
     return out
 
 
@@ -132,7 +139,7 @@ def mxfp4_expert_dense(x, w, plan, bias=None, activation=None, out_dtype=None, s
     if x.dim() != 2 or x.shape[0] != want:
         raise ValueError(f'x must be [{want}, {w.k}], got {tuple(x.shape)}')
     out = x.new_empty((plan.n_rows, w.rows), dtype=out_dtype)
-    nbytes = _lib.lib.gunet_mxfp4_dense_workspace_bytes(plan.n_rows, w.k)
+    nbytes = _lib.lib.gunet_mxfp4_expert_dense_workspace_bytes(plan.n_rows, w.k)
     scratch = w.codes.new_empty(nbytes)
     launch('gunet_mxfp4_expert_dense_forward', w.device, x.data_ptr(), code, plan.offsets.data_ptr(),
            None if sorted_rows else plan.slot.data_ptr(), plan.n_tokens, plan.top_k, plan.n_experts, w.k, w.codes.data_ptr(),

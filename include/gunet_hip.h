@@ -432,8 +432,8 @@ int gunet_mxfp4_dequantize(const uint8_t* codes, const uint8_t* scales, int64_t 
  * column: the transpose of a Dense kernel), n_out >= 1.  Products are exact (below 2^-126 they may be 0), sums float32; the bias (float32 [n_out] or NULL) is added last,
  * then the activation, then one rounding to out_dtype.  A linear layer hands a NaN on, the ReLU of a NaN is 0
  * as in the float32 layers.  Independent of the matmul mode.  The order of the sums depends on the sizes, not on the run.
- * workspace: the quantised x, gunet_mxfp4_dense_workspace_bytes(rows, k) bytes, 16-byte aligned; calls that may overlap in
- * time need one each. */
+ * workspace: the quantised x, gunet_mxfp4_dense_workspace_bytes(rows, k) bytes, 16-byte aligned (0 for little x, which is
+ * quantised inside the product: NULL then); calls that may overlap in time need one each. */
 size_t gunet_mxfp4_dense_workspace_bytes(int64_t rows, int32_t k);
 int gunet_mxfp4_dense_forward(const void* x, int32_t dtype, int64_t rows, int32_t k, const uint8_t* w_codes,
                               const uint8_t* w_scales, const float* bias, int32_t n_out, int32_t activation, void* out,
@@ -442,8 +442,9 @@ int gunet_mxfp4_dense_forward(const void* x, int32_t dtype, int64_t rows, int32_
 /* The experts' Dense layers: out[r] = act(q(row r) @ w[e]^T + bias[e]) for the rows r of expert e, zeros behind
  * offsets[n_experts].  With slot: x [n_tokens, k], row r is the token whose choice has slot r (the dispatch happens on the 4-bit
  * rows); slot = NULL: x [n_tokens * top_k, k] is in expert order already.  w [n_experts, n_out, k], bias float32 [n_experts, n_out]
- * or NULL, out [n_tokens * top_k, n_out].  workspace: gunet_mxfp4_dense_workspace_bytes(n_tokens * top_k, k) bytes, 16-byte
- * aligned. */
+ * or NULL, out [n_tokens * top_k, n_out].  workspace: gunet_mxfp4_expert_dense_workspace_bytes(n_tokens * top_k, k) bytes,
+ * 16-byte aligned. */
+size_t gunet_mxfp4_expert_dense_workspace_bytes(int64_t rows, int32_t k);
 int gunet_mxfp4_expert_dense_forward(const void* x, int32_t dtype, const int32_t* offsets, const int32_t* slot,
                                      int64_t n_tokens, int32_t top_k, int32_t n_experts, int32_t k, const uint8_t* w_codes,
                                      const uint8_t* w_scales, const float* bias, int32_t n_out, int32_t activation, void* out,

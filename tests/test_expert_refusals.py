@@ -77,13 +77,14 @@ def test_mxfp4(lib):
 
 
 def test_products(lib):
-    need = lib.gunet_mxfp4_dense_workspace_bytes(4, 64)
-    assert need == 256 + 4 * 8
+    assert lib.gunet_mxfp4_dense_workspace_bytes(40, 64) == 40 * 32 + 40 * 8 and lib.gunet_mxfp4_dense_workspace_bytes(4, 64) == 0
+    need = lib.gunet_mxfp4_dense_workspace_bytes(40, 64)
+    assert lib.gunet_mxfp4_expert_dense_workspace_bytes(4, 64) == 256 + 4 * 8
 
-    def dense(x=P, dtype=0, rows=4, k=64, wc=P, ws=P, bias=None, n=8, act=0, out=P, out_dtype=0, scratch=P, nbytes=1 << 30):
+    def dense(x=P, dtype=0, rows=40, k=64, wc=P, ws=P, bias=None, n=8, act=0, out=P, out_dtype=0, scratch=P, nbytes=1 << 30):
         return lib.gunet_mxfp4_dense_forward(x, dtype, rows, k, wc, ws, bias, n, act, out, out_dtype, scratch, nbytes, None)
 
-    def expert(x=P, dtype=0, offsets=P, slot=P, rows=4, top_k=2, e=3, k=64, wc=P, ws=P, bias=None, n=8, act=0, out=P, out_dtype=0, scratch=P, nbytes=1 << 30):
+    def expert(x=P, dtype=0, offsets=P, slot=P, rows=20, top_k=2, e=3, k=64, wc=P, ws=P, bias=None, n=8, act=0, out=P, out_dtype=0, scratch=P, nbytes=1 << 30):
         return lib.gunet_mxfp4_expert_dense_forward(x, dtype, offsets, slot, rows, top_k, e, k, wc, ws, bias, n, act, out, out_dtype, scratch, nbytes, None)
 
     for fn in (dense, expert):
@@ -94,7 +95,8 @@ def test_products(lib):
         assert fn(rows=0) == OK
     for kw in (dict(offsets=None), dict(top_k=0), dict(e=0), dict(rows=2 ** 30, top_k=2), dict(e=65536)):
         assert expert(**kw) == INVALID, kw
-    assert expert(nbytes=lib.gunet_mxfp4_dense_workspace_bytes(8, 64) - 1) == WORKSPACE
+    assert expert(nbytes=lib.gunet_mxfp4_expert_dense_workspace_bytes(40, 64) - 1) == WORKSPACE
+    assert expert(rows=2, nbytes=lib.gunet_mxfp4_expert_dense_workspace_bytes(4, 64) - 1) == WORKSPACE
 
 
 def test_python_checks_need_no_gpu():
