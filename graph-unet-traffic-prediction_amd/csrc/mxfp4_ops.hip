@@ -48,11 +48,15 @@ struct QuantArgs {
 // Eight elements of a row from column `col` on (columns past k read as 0): the lane's share of its block.
 template <typename T, bool VEC>
 __device__ __forceinline__ void load_eight(const T* row, int col, int k, float (&v)[8]) {
-  if (VEC && col + 8 <= k) {
+  if (col + 8 <= k) {
     constexpr int kPer = 16 / sizeof(T);
 #pragma unroll
     for (int p = 0; p < 8 / kPer; ++p) {
-      const Pack<T, kPer> q = load_pack<T, kPer>(row + col + p * kPer);
+      Pack<T, kPer> q;
+      if (VEC)
+        q = load_pack<T, kPer>(row + col + p * kPer);
+      else
+        __builtin_memcpy(&q, row + col + p * kPer, sizeof(q));     // an unaligned load
 #pragma unroll
       for (int c = 0; c < kPer; ++c) v[p * kPer + c] = to_f32(q.v[c]);
     }
@@ -118,44 +122,45 @@ __global__ __launch_bounds__(kThreads) void k_mxfp4_quantize(QuantArgs a, const 
   }
 }
 
+// The inverse: a lane writes 16 bytes, 4 or 8 values of one block (8 float32 values a lane, in two stores whose lanes lie 32 bytes apart, took
+// 35 us for 4096 x 8192 where this takes 27.6, 5.5 TB/s).  Rows that do not start on 16 bytes: unaligned stores, 28.5 us at 8191.
 template <typename T>
 __global__ __launch_bounds__(kThreads) void k_mxfp4_dequantize(int64_t rows, int32_t k, int32_t blocks, const uint8_t* __restrict__ codes,
                                                                const uint8_t* __restrict__ scales, T* __restrict__ out) {
-  const int64_t parts = static_cast<int64_t>(blocks) * 4;
+  constexpr int kPer = 16 / sizeof(T);
+  using Word = typename std::conditional<kPer == 8, uint32_t, uint16_t>::type;
+  const int64_t parts = static_cast<int64_t>(blocks) * (kBlock / kPer);
   const int64_t group = blockIdx.y;
   out += group * rows * k;
   codes += group * rows * blocks * 16;
   scales += group * ((blocks + kTileBlocks - 1) / kTileBlocks) * rows * 8;
-  const bool vec = k % 8 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0;
+  const bool vec = k % kPer == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0;
   for (int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; i < rows * parts; i += static_cast<int64_t>(gridDim.x) * kThreads) {
     const int64_t row = i / parts;
     const int part = static_cast<int>(i - row * parts);
-    const int block = part >> 2, col = part * 8;
-    const uint32_t word = reinterpret_cast<const uint32_t*>(codes)[i];
+    const int block = part / (kBlock / kPer), col = part * kPer;
+    const uint32_t word = reinterpret_cast<const Word*>(codes)[i];
     const uint32_t byte = scales[(static_cast<int64_t>(block / kTileBlocks) * rows + row) * 8 + block % kTileBlocks];
-    const float s = scale_value(byte);
+    const float s = scale_value(byte), nan = __uint_as_float(0x7FC00000u);
     const auto v0 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(word, s, 0);
     const auto v1 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(word, s, 1);
-    const auto v2 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(word, s, 2);
-    const auto v3 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(word, s, 3);
-    const float nan = __uint_as_float(0x7FC00000u);
-    const float v[8] = {v0[0], v0[1], v1[0], v1[1], v2[0], v2[1], v3[0], v3[1]};
-    Pack<T, 8> o;
+    float v[8] = {v0[0], v0[1], v1[0], v1[1]};
+    if (kPer == 8) {
+      const auto v2 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(word, s, 2);
+      const auto v3 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(word, s, 3);
+      v[4] = v2[0], v[5] = v2[1], v[6] = v3[0], v[7] = v3[1];
+    }
+    Pack<T, kPer> o;
 #pragma unroll
-    for (int c = 0; c < 8; ++c) o.v[c] = from_f32<T>(byte == 255 ? nan : v[c]);
+    for (int c = 0; c < kPer; ++c) o.v[c] = from_f32<T>(byte == 255 ? nan : v[c]);
     T* const dst = out + row * k + col;
-    if (vec && col + 8 <= k) {
-      constexpr int kPer = 16 / sizeof(T);
-#pragma unroll
-      for (int p = 0; p < 8 / kPer; ++p) {
-        Pack<T, kPer> q;
-#pragma unroll
-        for (int c = 0; c < kPer; ++c) q.v[c] = o.v[p * kPer + c];
-        store_pack<T, kPer>(dst + p * kPer, q);
-      }
+    if (vec) {
+      if (col < k) store_pack<T, kPer>(dst, o);      // k is a multiple of kPer: all of the piece or none
+    } else if (col + kPer <= k) {
+      __builtin_memcpy(dst, &o, sizeof(o));          // an unaligned store
     } else {
 #pragma unroll
-      for (int c = 0; c < 8; ++c)
+      for (int c = 0; c < kPer; ++c)
         if (col + c < k) dst[c] = o.v[c];
     }
   }
@@ -709,28 +714,34 @@ int launch_raw(const ProductArgs& a, hipStream_t stream) {
 // Which form.  Rows per group decide how many rows a tile can fill, the number of tiles whether they fill the chip (256 CUs).
 // Measured, product alone (us):
 //   rows x k x n         16 columns a workgroup   64 x 64   128 x 128   256 x 256
-//   1 x 4096 x 4096              3.4                8.5       12.8        27.6
-//   32 x 4096 x 4096             5.6                8.6
-//   64 x 4096 x 4096             8.1                8.7       13.8        28.2
-//   256 x 4096 x 4096           24.3                9.8
-//   2048 x 8192 x 1024                             20.6       26.7        52.0
-//   1024 x 2048 x 4096                             15.9       11.9        20.9
-//   48332 x 256 x 256                              19.9       11.9        13.2
-//   4096 x 4096 x 4096                             84.5       50.6        43.1
-//   8192 x 8192 x 8192                              590        381         328
-// and for 32 experts 2048 -> 4096 (quantisation included), average rows per expert 4 / 8 / 32: 16 columns 28.5 / 35.1 / 79, 64 x 64 36.8 / 38.8 / 49.
+//   1 x 4096 x 4096              3.4                7.6       12.4        26.4
+//   32 x 4096 x 4096             5.7                7.7       13.0        26.7
+//   64 x 4096 x 4096             8.6                7.8       13.3        26.6
+//   256 x 4096 x 4096           26.5                8.9       14.3        27.6
+//   2048 x 8192 x 1024                             18.8       25.1        48.6
+//   1024 x 2048 x 4096                             13.6       10.5        18.1
+//   48332 x 256 x 256                              16.4       10.5         9.9
+//   4096 x 4096 x 4096                             79.8       48.5        37.7
+//   8192 x 8192 x 8192                              540        326         258
+// and 32 experts 2048 -> 4096 with their quantisation, by average rows per expert:
+//   4                           35.5               39.7       39.3        48.5
+//   8                           42.2               41.4       41.1        49.2
+//   64                           147               57.5       53.9        58.4
+//   128                          269               86.4       62.2        69.1
+//   256                          492                152        102        91.3
 int launch_product(ProductArgs a, hipStream_t stream) {
   a.out_wide = reinterpret_cast<uintptr_t>(a.out) % 16 == 0 && a.n_out * dtype_size(a.out_dtype) % 16 == 0;
   const int64_t per_group = a.offsets ? ceil_div(a.rows, a.groups) : a.rows;
   const auto tiles = [&](int64_t size) { return (a.rows / size + (a.offsets ? a.groups / 2 : 1)) * ceil_div(a.n_out, size); };
-  if (per_group <= (a.offsets ? 8 : 16)) {
-    // two waves a workgroup stream as well as four once there are four workgroups per CU, and leave more of them side by side (1.18x)
+  if (per_group <= (a.offsets ? 6 : 16)) {
+    // two waves a workgroup stream as well as four once there are four workgroups per CU, and leave more of them side by side: 35.5 us
+    // against 41.6 in the experts' first line
     if (std::min<int64_t>(a.rows, a.rows / 16 + a.groups) * ceil_div(a.n_out, 16) >= 1024) return launch_skinny<1, 2>(a, stream);
     return launch_skinny<1, 4>(a, stream);
   }
   if (a.offsets == nullptr && a.rows <= 32) return launch_skinny<2, 4>(a, stream);
   if (per_group >= 256 && tiles(256) >= 256) return launch_tile<2, 4, 4, 2, 2>(a, stream);
-  if (per_group >= 96 && tiles(128) >= 256) return launch_tile<2, 4, 2, 1, 2>(a, stream);
+  if ((a.offsets || a.rows >= 96) && tiles(128) >= 256) return launch_tile<2, 4, 2, 1, 2>(a, stream);
   return launch_tile<2, 2, 1, 1, 4>(a, stream);
 }
 
@@ -825,7 +836,7 @@ int gunet_mxfp4_dequantize(const uint8_t* codes, const uint8_t* scales, int64_t 
                     reinterpret_cast<uintptr_t>(out) % dtype_size(dtype) == 0,
                 "mxfp4_dequantize: codes must lie on 16 bytes, scales on 8, out on its type's size");
   const int32_t blocks = static_cast<int32_t>(blocks_of(k));
-  const dim3 grid(stride_grid(rows * blocks * 4), static_cast<unsigned>(groups));
+  const dim3 grid(stride_grid(rows * blocks * (dtype == GUNET_DTYPE_F32 ? 8 : 4)), static_cast<unsigned>(groups));
   hipStream_t s = as_stream(stream);
   if (dtype == GUNET_DTYPE_F32)
     k_mxfp4_dequantize<float><<<grid, kThreads, 0, s>>>(rows, k, blocks, codes, scales, static_cast<float*>(out));
