@@ -279,8 +279,10 @@ __device__ __forceinline__ v16f mfma_fp4(uint4 a, uint4 b, v16f c, int step, int
 
 // 16 bytes per lane from memory straight into LDS: lane l's land at lds_base + 16 l.  The compiler does not see the load: the caller
 // waits for it before a barrier.  What lies out of the buffer's range reads as zeros.
+// The compiler does not look into the asm for hazards either: m0 has to be written one wait state before a load to LDS, and scalar registers
+// that the vector unit wrote (readfirstlane) five before a load that reads them.
 __device__ __forceinline__ void dma_to_lds(u32x4 rsrc, uint32_t lds_base, uint32_t lane_off, uint32_t uniform_off) {
-  asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(lds_base), "v"(lane_off), "s"(rsrc), "s"(uniform_off)
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(lds_base), "v"(lane_off), "s"(rsrc), "s"(uniform_off)
                : "memory", "m0");
 }
 // Waits until at most N of this wave's loads are on their way and its LDS reads are done, then for the other waves.
