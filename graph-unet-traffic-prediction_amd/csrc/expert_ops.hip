@@ -201,10 +201,10 @@ __device__ __forceinline__ int64_t kept_row(int32_t s, int64_t n_rows) { return 
 template <typename T>
 constexpr int kVec = 16 / sizeof(T);
 
-template <typename T, int N, bool FULL>
+template <typename T, int N, bool FULL, bool ONCE = false>
 __device__ __forceinline__ Pack<T, N> load_piece(const T* row, int piece, int width) {
   const T* const p = row + static_cast<int64_t>(piece) * N;
-  if (FULL) return load_pack<T, N>(p);
+  if (FULL) return ONCE ? load_pack_once<T, N>(p) : load_pack<T, N>(p);
   Pack<T, N> v = {};
   if (piece * N + N <= width) {
     __builtin_memcpy(&v, p, sizeof(v));
@@ -240,7 +240,7 @@ __device__ __forceinline__ void zero_tail(const RowArgs& a, T* rows) {
 }
 
 // rows[slot[t][j]] = x[t]: a token's row is read once and written top_k times.  HBM-bound: (n_tokens + n) rows.
-template <typename T, int N>
+template <typename T, int N, bool ONCE>
 __global__ __launch_bounds__(kThreads) void k_expert_dispatch(RowArgs a, const T* __restrict__ x, T* __restrict__ rows) {
   constexpr int U = 4;
   const int lanes = 1 << a.lanes_log2;
@@ -252,7 +252,7 @@ __global__ __launch_bounds__(kThreads) void k_expert_dispatch(RowArgs a, const T
       Pack<T, N> v[U];
 #pragma unroll
       for (int i = 0; i < U; ++i)
-        if (u + i * lanes < a.pieces) v[i] = load_piece<T, N, true>(src, u + i * lanes, a.width);
+        if (u + i * lanes < a.pieces) v[i] = load_piece<T, N, true, ONCE>(src, u + i * lanes, a.width);
       for (int j = 0; j < a.top_k; ++j) {
         const int64_t r = kept_row(a.slot[t * a.top_k + j], a.n_rows);
         if (r < 0) continue;
@@ -267,7 +267,7 @@ __global__ __launch_bounds__(kThreads) void k_expert_dispatch(RowArgs a, const T
 
 // out[t] = sum_j weights[t][j] rows[slot[t][j]] (WEIGHTED), or the plain sum: combine, and dispatch's gradient.
 // Four choices' pieces are fetched together, U of each; the sum is float32, choice 0 first, rounded once.
-template <typename T, bool FULL, bool WEIGHTED, int U>
+template <typename T, bool FULL, bool WEIGHTED, int U, bool ONCE>
 __global__ __launch_bounds__(kThreads) void k_expert_combine(RowArgs a, const T* __restrict__ rows, const float* __restrict__ weights,
                                                              T* __restrict__ out) {
   constexpr int N = kVec<T>;
@@ -289,7 +289,7 @@ __global__ __launch_bounds__(kThreads) void k_expert_combine(RowArgs a, const T*
           w[j] = WEIGHTED ? weights[t * a.top_k + j0 + j] : 1.0f;
 #pragma unroll
           for (int i = 0; i < U; ++i)
-            if (u + i * lanes < a.pieces) v[j][i] = load_piece<T, N, FULL>(rows + r * a.width, u + i * lanes, a.width);
+            if (u + i * lanes < a.pieces) v[j][i] = load_piece<T, N, FULL, ONCE>(rows + r * a.width, u + i * lanes, a.width);
         }
 #pragma unroll
         for (int j = 0; j < 4; ++j)
@@ -331,7 +331,7 @@ __device__ __forceinline__ float sum_over_lanes(float v, int lanes) {
 // Combine's gradient: grad_rows[slot[t][j]] = weights[t][j] grad[t], grad_weights[t][j] = <grad[t], rows[slot[t][j]]>
 // (0 where the choice was dropped).  One pass: a token's gradient is read once per four choices, each choice's row read once
 // and its gradient written once.  The dot product is a float32 sum per lane, then a fixed tree over the lanes.
-template <typename T, int N, int U>
+template <typename T, int N, int U, bool ONCE>
 __global__ __launch_bounds__(kThreads) void k_expert_combine_grad(RowArgs a, const T* __restrict__ grad, const T* __restrict__ rows,
                                                                   const float* __restrict__ weights, T* __restrict__ grad_rows,
                                                                   float* __restrict__ grad_weights) {
@@ -351,13 +351,13 @@ __global__ __launch_bounds__(kThreads) void k_expert_combine_grad(RowArgs a, con
         Pack<T, N> g[U], v[4][U];
 #pragma unroll
         for (int i = 0; i < U; ++i)
-          if (u + i * lanes < a.pieces) g[i] = load_piece<T, N, true>(grad + t * a.width, u + i * lanes, a.width);
+          if (u + i * lanes < a.pieces) g[i] = load_piece<T, N, true, ONCE>(grad + t * a.width, u + i * lanes, a.width);
 #pragma unroll
         for (int j = 0; j < 4; ++j)
           if (r[j] >= 0)
 #pragma unroll
             for (int i = 0; i < U; ++i)
-              if (u + i * lanes < a.pieces) v[j][i] = load_piece<T, N, true>(rows + r[j] * a.width, u + i * lanes, a.width);
+              if (u + i * lanes < a.pieces) v[j][i] = load_piece<T, N, true, ONCE>(rows + r[j] * a.width, u + i * lanes, a.width);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           if (r[j] < 0) continue;
@@ -436,8 +436,16 @@ int by_type(int32_t dtype, int64_t width, std::initializer_list<const void*> ptr
 }
 
 // Rows of that many pieces are worked on two pieces a lane at a time: combine of 16384 x 4 rows of 2048 bf16 76 us against 83, of 4096 x 2 rows
-// of 1024 4.9 against 5.3 (256 float32, 64 pieces: 66 against 52); combine's gradient 146 against 153, but 12.3 against 9.2 at 128 pieces.
+// of 1024 4.9 against 5.3 (256 float32, 64 pieces: 66 against 52); combine's gradient from twice as many on: 146 against 153, but
+// 12.3 against 9.2 at 128 pieces.
 constexpr int kWidePieces = 128;
+
+// Where the rows are more than the L2s hold (8 x 4 MB) everything is read past the caches, which are then left to what is written.  bf16 rows of 1 KB,
+// combine / its gradient (us): 8 MB 5.9 / 8.1 against 5.1 / 7.2 through the caches, 32 MB 11.1 / 19.1 against 13.9 / 19.1, 200 MB 51.5 / 88
+// against 53.6 / 101, 400 MB 98 / 194 against 107 / 194; 16384 x 4 rows of 4 KB dispatched 54 against 67, combine's gradient 112 against 134.
+bool read_once(const RowArgs& a, int32_t dtype) {
+  return a.n_rows * a.width * static_cast<int64_t>(dtype_size(dtype)) >= (int64_t{32} << 20);
+}
 
 int key_bits_of(int n_experts) {
   int bits = 0;
@@ -457,7 +465,9 @@ int run_combine(const char* fn, const void* rows, int32_t dtype, const float* we
     using T = typename Tag::type;
     constexpr bool kFull = Tag::vec == kVec<T>;
     const RowArgs a = row_args(n_tokens, top_k, 0, width, kVec<T>, slot, nullptr);
-    auto* const kernel = a.pieces >= kWidePieces ? &k_expert_combine<T, kFull, WEIGHTED, 2> : &k_expert_combine<T, kFull, WEIGHTED, 1>;
+    const bool wide = a.pieces >= kWidePieces, once = kFull && read_once(a, dtype);
+    auto* const kernel = wide ? (once ? &k_expert_combine<T, kFull, WEIGHTED, 2, kFull> : &k_expert_combine<T, kFull, WEIGHTED, 2, false>)
+                              : (once ? &k_expert_combine<T, kFull, WEIGHTED, 1, kFull> : &k_expert_combine<T, kFull, WEIGHTED, 1, false>);
     kernel<<<row_grid(a), kThreads, 0, as_stream(stream)>>>(a, static_cast<const T*>(rows), weights, static_cast<T*>(out));
     GUNET_LAUNCH_CHECK();
     return GUNET_OK;
@@ -521,7 +531,9 @@ int gunet_expert_dispatch(const void* x, int32_t dtype, const int32_t* offsets, 
     using Tag = decltype(tag);
     using T = typename Tag::type;
     const RowArgs a = row_args(n_tokens, top_k, n_experts, width, Tag::vec, slot, offsets);
-    k_expert_dispatch<T, Tag::vec><<<row_grid(a), kThreads, 0, as_stream(stream)>>>(a, static_cast<const T*>(x), static_cast<T*>(rows));
+    constexpr bool kFull = Tag::vec == kVec<T>;
+    auto* const kernel = kFull && read_once(a, dtype) ? &k_expert_dispatch<T, Tag::vec, kFull> : &k_expert_dispatch<T, Tag::vec, false>;
+    kernel<<<row_grid(a), kThreads, 0, as_stream(stream)>>>(a, static_cast<const T*>(x), static_cast<T*>(rows));
     GUNET_LAUNCH_CHECK();
     return GUNET_OK;
   });
@@ -552,8 +564,11 @@ int gunet_expert_combine_grad(const void* grad_out, const void* rows, int32_t dt
     using Tag = decltype(tag);
     using T = typename Tag::type;
     const RowArgs a = row_args(n_tokens, top_k, n_experts, width, Tag::vec, slot, offsets);
-    constexpr int kWide = Tag::vec == kVec<T> ? 2 : 1;
-    auto* const kernel = a.pieces >= 2 * kWidePieces ? &k_expert_combine_grad<T, Tag::vec, kWide> : &k_expert_combine_grad<T, Tag::vec, 1>;
+    constexpr bool kFull = Tag::vec == kVec<T>;
+    constexpr int kWide = kFull ? 2 : 1;
+    const bool wide = a.pieces >= 2 * kWidePieces, once = kFull && read_once(a, dtype);
+    auto* const kernel = wide ? (once ? &k_expert_combine_grad<T, Tag::vec, kWide, kFull> : &k_expert_combine_grad<T, Tag::vec, kWide, false>)
+                              : (once ? &k_expert_combine_grad<T, Tag::vec, 1, kFull> : &k_expert_combine_grad<T, Tag::vec, 1, false>);
     kernel<<<row_grid(a), kThreads, 0, as_stream(stream)>>>(
         a, static_cast<const T*>(grad_out), static_cast<const T*>(rows), weights, static_cast<T*>(grad_rows), grad_weights);
     GUNET_LAUNCH_CHECK();

@@ -31,6 +31,16 @@ __device__ __forceinline__ void store_pack(T* p, const Pack<T, VEC>& v) {
   *reinterpret_cast<Pack<T, VEC>*>(p) = v;
 }
 
+// load_pack for what is read once: past the caches, which keep what is read again and written.
+template <typename T, int VEC>
+__device__ __forceinline__ Pack<T, VEC> load_pack_once(const T* p) {
+  using P = Pack<T, VEC>;
+  if constexpr (sizeof(P) == 16)
+    return __builtin_bit_cast(P, __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p)));
+  else
+    return load_pack<T, VEC>(p);
+}
+
 template <typename T>
 __device__ __forceinline__ float to_f32(T v) {
   return static_cast<float>(v);

@@ -123,7 +123,7 @@ __global__ __launch_bounds__(kThreads) void k_mxfp4_quantize(QuantArgs a, const 
 }
 
 // The inverse: a lane writes 16 bytes, 4 or 8 values of one block (8 float32 values a lane, in two stores whose lanes lie 32 bytes apart, took
-// 35 us for 4096 x 8192 where this takes 27.6, 5.5 TB/s).  Rows that do not start on 16 bytes: unaligned stores, 28.5 us at 8191.
+// 35 us for 4096 x 8192 where this takes 27.6, 5.5 TB/s), past the caches (quantised and read back 57.6 us against 63).  Rows that do not start on 16 bytes: unaligned stores, 28.5 us at 8191.
 template <typename T>
 __global__ __launch_bounds__(kThreads) void k_mxfp4_dequantize(int64_t rows, int32_t k, int32_t blocks, const uint8_t* __restrict__ codes,
                                                                const uint8_t* __restrict__ scales, T* __restrict__ out) {
@@ -154,8 +154,8 @@ __global__ __launch_bounds__(kThreads) void k_mxfp4_dequantize(int64_t rows, int
 #pragma unroll
     for (int c = 0; c < kPer; ++c) o.v[c] = from_f32<T>(byte == 255 ? nan : v[c]);
     T* const dst = out + row * k + col;
-    if (vec) {
-      if (col < k) store_pack<T, kPer>(dst, o);      // k is a multiple of kPer: all of the piece or none
+    if (vec) {      // k is a multiple of kPer: all of the piece or none
+      if (col < k) __builtin_nontemporal_store(__builtin_bit_cast(u32x4, o), reinterpret_cast<u32x4*>(dst));
     } else if (col + kPer <= k) {
       __builtin_memcpy(dst, &o, sizeof(o));          // an unaligned store
     } else {
