@@ -19,6 +19,7 @@ ACT_TANH, ACT_SIGMOID, ACT_ELU, ACT_SOFTPLUS, ACT_SELU, ACT_SWISH = 2, 3, 4, 5, 
 ACT_GELU, ACT_SOFTSIGN, ACT_EXPONENTIAL, ACT_HARD_SIGMOID = 8, 9, 10, 11
 
 DTYPE_F32, DTYPE_BF16, DTYPE_F16 = 0, 1, 2
+MAX_EXPERTS = 1024
 
 MATMUL_MODES = {'f32': 0, 'split3': 1, 'split2': 2, 'bf16': 3}
 

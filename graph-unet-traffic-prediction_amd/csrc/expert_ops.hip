@@ -18,7 +18,8 @@ constexpr int kSortWaves = kSortThreads / 64;
 constexpr int kSortPerThread = 2;
 constexpr int kSortTile = kSortThreads * kSortPerThread;   // flat positions one round of a workgroup ranks
 constexpr int kSortMaxBlocks = 256;
-constexpr int kMaxExperts = 1024;                          // one thread per expert in the scans
+constexpr int kMaxExperts = GUNET_MAX_EXPERTS;             // one thread per expert in the scans
+static_assert(kMaxExperts <= kSortThreads, "one thread per expert");
 constexpr int kThreads = 256;
 
 struct SortShape {

@@ -67,7 +67,7 @@ def expert_plan(expert_index, n_experts):
     n_experts = int(n_experts)
     t, k = index.shape
     dev = index.device
-    offsets = index.new_empty(max(n_experts, 0) + 1)
+    offsets = index.new_empty(max(0, min(n_experts, _lib.MAX_EXPERTS)) + 1)       # the library refuses other numbers
     order = index.new_empty(t * k)
     slot = index.new_empty((t, k))
     nbytes = _lib.lib.gunet_expert_sort_workspace_bytes(t, k, n_experts)

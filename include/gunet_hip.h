@@ -381,13 +381,16 @@ int gunet_unet_forward_static_f32(const gunet_plan* plan, const gunet_unet_weigh
 #define GUNET_DTYPE_BF16 1
 #define GUNET_DTYPE_F16 2
 
+#define GUNET_MAX_EXPERTS 1024
+
 /* Stable counting sort of the n = n_tokens * top_k flat positions f = t * top_k + j by expert_index[t][j]
  * (int32 [n_tokens, top_k]).  A value outside 0 .. n_experts-1 is a dropped choice.
  *   offsets int32 [n_experts + 1]      rows offsets[e] .. offsets[e+1]-1 belong to expert e
  *   order   int32 [n]                  flat position of each row, ascending within an expert; -1 behind
  *                                      offsets[n_experts]
  *   slot    int32 [n_tokens, top_k]    the inverse: row of each flat position; -1 = dropped
- * A token may name one expert several times.  n <= 2^31 - 1; n_experts <= 1024 (else GUNET_ERR_UNSUPPORTED).
+ * A token may name one expert several times.  n <= 2^31 - 1; n_experts <= GUNET_MAX_EXPERTS (else
+ * GUNET_ERR_UNSUPPORTED).
  * workspace: 4-byte aligned; gunet_expert_sort_workspace_bytes may be 0, then it may be NULL. */
 size_t gunet_expert_sort_workspace_bytes(int64_t n_tokens, int32_t top_k, int32_t n_experts);
 int gunet_expert_sort(const int32_t* expert_index, int64_t n_tokens, int32_t top_k, int32_t n_experts, int32_t* offsets,

@@ -99,6 +99,17 @@ def test_products(lib):
     assert expert(rows=2, nbytes=lib.gunet_mxfp4_expert_dense_workspace_bytes(4, 64) - 1) == WORKSPACE
 
 
+def test_constants_match_the_header():
+    import os
+    import re
+    from conftest import ROOT
+    from gunet_amd import _lib
+    with open(os.path.join(ROOT, 'include', 'gunet_hip.h')) as f:
+        defines = dict(re.findall(r'#define\s+(GUNET_[A-Z0-9_]+)\s+\(?(-?\d+)\)?', f.read()))
+    assert [int(defines['GUNET_DTYPE_' + t]) for t in ('F32', 'BF16', 'F16')] == [_lib.DTYPE_F32, _lib.DTYPE_BF16, _lib.DTYPE_F16]
+    assert int(defines['GUNET_MAX_EXPERTS']) == _lib.MAX_EXPERTS
+
+
 def test_python_checks_need_no_gpu():
     import torch
     import gunet_amd as amd

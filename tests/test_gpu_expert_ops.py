@@ -262,6 +262,85 @@ def test_two_streams_at_once(amd):
         assert all(torch.equal(a, b) for a, b in zip(gots, wants))
 
 
+def test_two_host_threads_at_once(amd):
+    """Each thread on a stream of its own, all entry points: no state is shared."""
+    import threading
+    rng = np.random.default_rng(21)
+    cases = []
+    for s in range(2):
+        index = torch.as_tensor(_index(rng, 3000, 3, 9, 'dropped')).cuda()
+        x = torch.as_tensor(rng.standard_normal((3000, 72)), dtype=torch.float32).cuda()
+        w = torch.as_tensor(rng.random((3000, 3)), dtype=torch.float32).cuda()
+        cases.append((index, x, w))
+
+    def work(index, x, w):
+        plan = amd.expert_plan(index, 9)
+        rows = amd.expert_dispatch(x, plan)
+        return (amd.expert_combine(rows, w, plan),) + amd.expert_combine_grad(x, rows, w, plan)
+
+    wants = [work(*c) for c in cases]
+    torch.cuda.synchronize()
+    gots, failures = [[], []], []
+
+    def loop(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(20):
+                    gots[i] = work(*cases[i])
+            torch.cuda.synchronize()
+        except Exception as e:          # reported by the main thread
+            failures.append(e)
+
+    threads = [threading.Thread(target=loop, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failures
+    for got, want in zip(gots, wants):
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_as_autograd_functions(amd):
+    """The gradient functions inside torch's autograd, as a training step uses them, against the formula in 64 bits."""
+    class Dispatch(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, x, plan):
+            ctx.plan = plan
+            return amd.expert_dispatch(x, plan)
+
+        @staticmethod
+        @torch.autograd.function.once_differentiable
+        def backward(ctx, grad):
+            return amd.expert_dispatch_grad(grad, ctx.plan), None
+
+    class Combine(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, rows, weights, plan):
+            ctx.plan = plan
+            ctx.save_for_backward(rows, weights)
+            return amd.expert_combine(rows, weights, plan)
+
+        @staticmethod
+        @torch.autograd.function.once_differentiable
+        def backward(ctx, grad):
+            return (*amd.expert_combine_grad(grad, *ctx.saved_tensors, ctx.plan), None)
+
+    rng = np.random.default_rng(17)
+    t, k, e, width = 50, 3, 5, 24
+    plan = amd.expert_plan(torch.as_tensor(_index(rng, t, k, e, 'dropped')).cuda(), e)
+    x = torch.as_tensor(rng.standard_normal((t, width)), dtype=torch.float32).cuda().requires_grad_()
+    w = torch.as_tensor(rng.random((t, k)), dtype=torch.float32).cuda().requires_grad_()
+    Combine.apply(Dispatch.apply(x, plan) * 3, w, plan).sum().backward()      # .sum() hands back an expanded gradient
+    slot = plan.slot.cpu().numpy()
+    kept = slot >= 0
+    x64, w64 = x.detach().double().cpu().numpy(), w.detach().double().cpu().numpy()
+    want_x = np.repeat((3 * (w64 * kept).sum(1))[:, None], width, 1)
+    want_w = np.where(kept, 3 * x64.sum(1)[:, None], 0)
+    _near(x.grad, want_x, torch.float32, k + 2, 3 * np.abs(want_x))
+    _near(w.grad, want_w, torch.float32, width + 2, np.where(kept, 3 * np.abs(x64).sum(1)[:, None], 0))
+
+
 def test_refusals(amd):
     index = torch.zeros((4, 2), dtype=torch.int32).cuda()
     plan = amd.expert_plan(index, 3)
@@ -273,7 +352,7 @@ def test_refusals(amd):
     for bad in (index[0], index[:, :0]):
         with pytest.raises(ValueError):
             amd.expert_plan(bad, 3)
-    for e, code in ((0, -1), (-5, -1), (1025, -4)):
+    for e, code in ((0, -1), (-5, -1), (1025, -4), (2 ** 31 - 1, -4)):
         with pytest.raises(amd.GunetError) as err:
             amd.expert_plan(index, e)
         assert err.value.code == code
