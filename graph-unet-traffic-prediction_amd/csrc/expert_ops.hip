@@ -15,8 +15,11 @@ namespace {
 
 constexpr int kSortThreads = 1024;
 constexpr int kSortWaves = kSortThreads / 64;
-constexpr int kSortPerThread = 2;
-constexpr int kSortTile = kSortThreads * kSortPerThread;   // flat positions one round of a workgroup ranks
+// Flat positions per thread and round.  Up to 8192 positions one workgroup ranks all of them in one launch (9.4 us for 8192 of 8 experts; two
+// launches over tiles of 2048 take 7.6, but a launch costs the host 3.3); longer lists are cut into tiles of 2048, which more
+// workgroups share (65536 of 64 experts: 8.6 us, in tiles of 8192 15.0).
+constexpr int kSortAlone = 8, kSortShared = 2;
+constexpr int kSortTile = kSortThreads * kSortShared;
 constexpr int kSortMaxBlocks = 256;
 constexpr int kMaxExperts = GUNET_MAX_EXPERTS;             // one thread per expert in the scans
 static_assert(kMaxExperts <= kSortThreads, "one thread per expert");
@@ -24,14 +27,21 @@ constexpr int kThreads = 256;
 
 struct SortShape {
   int64_t blocks;   // workgroups
-  int64_t chunk;    // flat positions per workgroup, a multiple of kSortTile
+  int64_t chunk;    // flat positions per workgroup
+  bool alone;       // one workgroup, one round
 };
 
 // At most kSortMaxBlocks workgroups (each reads the counts of all others); longer lists make each of them
 // walk several tiles.
 SortShape sort_shape(int64_t n) {
   SortShape s;
-  const int64_t tiles = std::max<int64_t>(1, ceil_div(n, kSortTile));
+  s.alone = n <= kSortThreads * kSortAlone;
+  if (s.alone) {
+    s.chunk = kSortThreads * kSortAlone;
+    s.blocks = 1;
+    return s;
+  }
+  const int64_t tiles = ceil_div(n, kSortTile);
   const int64_t tiles_per_block = ceil_div(tiles, kSortMaxBlocks);
   s.chunk = tiles_per_block * kSortTile;
   s.blocks = ceil_div(tiles, tiles_per_block);
@@ -77,11 +87,12 @@ __global__ __launch_bounds__(kSortThreads) void k_expert_count(const int32_t* __
   for (int e = threadIdx.x; e < n_experts; e += kSortThreads) hist[static_cast<int64_t>(blockIdx.x) * n_experts + e] = lds[e];
 }
 
-// Ranks and writes one workgroup's chunk.  A wave owns 128 consecutive positions of a tile and ranks them 64 at
+// Ranks and writes one workgroup's chunk.  A wave owns 64 * PER consecutive positions of a tile and ranks them 64 at
 // a time: lanes with the same key find each other with one ballot per bit of the key, the lowest of them
 // claims the group's places from the wave's own counter of that expert.  Then the counters are summed over the
 // waves, offset by what earlier tiles, earlier workgroups and smaller experts hold, and every position has
-// its row.  Latency-bound: one launch up to kSortTile positions (hist unused), two above.
+// its row.  Latency-bound.  ALONE: all positions in one round of one workgroup, hist is not used.
+template <int PER, bool ALONE>
 __global__ __launch_bounds__(kSortThreads) void k_expert_rank(const int32_t* __restrict__ index, int64_t n, int64_t chunk, int n_experts,
                                                               int key_bits, const int32_t* __restrict__ hist,
                                                               int32_t* __restrict__ offsets, int32_t* __restrict__ order,
@@ -93,11 +104,10 @@ __global__ __launch_bounds__(kSortThreads) void k_expert_rank(const int32_t* __r
   int* const sums = before + n_experts;                  // [kSortWaves]
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
   const int64_t begin = blockIdx.x * chunk, end = begin + chunk < n ? begin + chunk : n;
-  const bool alone = gridDim.x == 1 && chunk == kSortTile;   // then the tile's own counts are all there is
 
   for (int e = t; e < n_experts; e += kSortThreads) base[e] = before[e] = 0;
   int total = 0;
-  if (!alone) {
+  if (!ALONE) {
     __syncthreads();
     // threads of one expert share the workgroups' counts out among them (integer sums: any order)
     int width = 1;
@@ -123,16 +133,16 @@ __global__ __launch_bounds__(kSortThreads) void k_expert_rank(const int32_t* __r
     if (blockIdx.x == 0 && t == 0) offsets[n_experts] = total;
   }
 
-  for (int64_t tile = begin; tile < end || (alone && tile == begin); tile += kSortTile) {
+  for (int64_t tile = begin; tile < end || (ALONE && tile == begin); tile += kSortThreads * PER) {
     __syncthreads();
     for (int i = t; i < kSortWaves * n_experts; i += kSortThreads) counts[i] = 0;
     __syncthreads();
-    int key[kSortPerThread], rank[kSortPerThread];
-    const int64_t at = tile + wave * (64 * kSortPerThread) + lane;
+    int key[PER], rank[PER];
+    const int64_t at = tile + wave * (64 * PER) + lane;
 #pragma unroll
-    for (int s = 0; s < kSortPerThread; ++s) key[s] = at + 64 * s < end ? clean_key(index[at + 64 * s], n_experts) : -1;
+    for (int s = 0; s < PER; ++s) key[s] = at + 64 * s < end ? clean_key(index[at + 64 * s], n_experts) : -1;
 #pragma unroll
-    for (int s = 0; s < kSortPerThread; ++s) {
+    for (int s = 0; s < PER; ++s) {
       rank[s] = 0;
       if (__any(key[s] >= 0)) {
         unsigned long long same = __ballot(key[s] >= 0);
@@ -156,7 +166,7 @@ __global__ __launch_bounds__(kSortThreads) void k_expert_rank(const int32_t* __r
         mine += c;
       }
     }
-    if (alone) {
+    if (ALONE) {
       const int first = block_exclusive(mine, sums, &total);
       if (t < n_experts) {
         base[t] = first;
@@ -166,7 +176,7 @@ __global__ __launch_bounds__(kSortThreads) void k_expert_rank(const int32_t* __r
     }
     __syncthreads();
 #pragma unroll
-    for (int s = 0; s < kSortPerThread; ++s) {
+    for (int s = 0; s < PER; ++s) {
       const int64_t i = at + 64 * s;
       if (i >= end) continue;
       int row = -1;
@@ -485,7 +495,7 @@ extern "C" {
 size_t gunet_expert_sort_workspace_bytes(int64_t n_tokens, int32_t top_k, int32_t n_experts) {
   if (check_shape("expert_sort", n_tokens, top_k, n_experts) != GUNET_OK || n_experts > kMaxExperts) return 0;
   const SortShape s = sort_shape(n_tokens * top_k);
-  return s.blocks == 1 && s.chunk == kSortTile ? 0 : static_cast<size_t>(s.blocks) * n_experts * sizeof(int32_t);
+  return s.alone ? 0 : static_cast<size_t>(s.blocks) * n_experts * sizeof(int32_t);
 }
 
 int gunet_expert_sort(const int32_t* expert_index, int64_t n_tokens, int32_t top_k, int32_t n_experts, int32_t* offsets, int32_t* order,
@@ -507,15 +517,17 @@ int gunet_expert_sort(const int32_t* expert_index, int64_t n_tokens, int32_t top
   GUNET_REQUIRE(need == 0 || reinterpret_cast<uintptr_t>(workspace) % 4 == 0, "expert_sort: workspace is not 4-byte aligned");
   int32_t* const hist = static_cast<int32_t*>(workspace);
   const unsigned grid = static_cast<unsigned>(s.blocks);
-  if (need > 0) {
+  if (!s.alone) {
     k_expert_count<<<grid, kSortThreads, n_experts * sizeof(int), as_stream(stream)>>>(expert_index, n, s.chunk, n_experts, hist);
     GUNET_LAUNCH_CHECK();
   }
   const size_t lds = (static_cast<size_t>(kSortWaves + 2) * n_experts + kSortWaves) * sizeof(int);
+  auto* const rank = !s.alone         ? &k_expert_rank<kSortShared, false>
+                     : n <= kSortTile ? &k_expert_rank<kSortShared, true>      // one token: 3.5 us against 4.0 with eight rounds to skip
+                                      : &k_expert_rank<kSortAlone, true>;
   if (lds > (size_t{64} << 10))   // 910 experts and more
-    GUNET_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void*>(&k_expert_rank), hipFuncAttributeMaxDynamicSharedMemorySize,
-                                      static_cast<int>(lds)));
-  k_expert_rank<<<grid, kSortThreads, lds, as_stream(stream)>>>(expert_index, n, s.chunk, n_experts, key_bits_of(n_experts), hist, offsets,
+    GUNET_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void*>(rank), hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lds)));
+  rank<<<grid, kSortThreads, lds, as_stream(stream)>>>(expert_index, n, s.chunk, n_experts, key_bits_of(n_experts), hist, offsets,
                                                                order, slot);
   GUNET_LAUNCH_CHECK();
   return GUNET_OK;

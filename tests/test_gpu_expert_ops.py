@@ -45,7 +45,7 @@ def _near(got, want, dtype, terms, size):
 
 
 @pytest.mark.parametrize('t, k, e', [(1, 1, 1), (1, 8, 64), (2, 3, 2), (63, 1, 5), (64, 2, 8), (65, 5, 7), (1000, 4, 128), (4096, 2, 8),
-                                     (4097, 2, 1024), (3001, 3, 1000), (9000, 4, 33), (20000, 6, 64)])
+                                     (4097, 2, 1024), (8193, 1, 16), (16384, 1, 8), (3001, 3, 1000), (9000, 4, 33), (20000, 6, 64)])
 @pytest.mark.parametrize('pattern', ['even', 'dropped', 'none', 'one', 'descending'])
 def test_sort_is_the_stable_order(amd, t, k, e, pattern):
     index = _index(np.random.default_rng(t + k + e), t, k, e, pattern)
