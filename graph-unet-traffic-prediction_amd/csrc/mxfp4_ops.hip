@@ -731,6 +731,10 @@ int launch_raw(const ProductArgs& a, hipStream_t stream) {
 //   64                           147               57.5       53.9        58.4
 //   128                          269               86.4       62.2        69.1
 //   256                          492                152        102        91.3
+// A CU takes in about 50 bytes a ns whatever the form, so a product of few tiles gains by smaller ones as long as each has a CU of its
+// own: 32 rows x 16 columns, eight waves sharing K, against 64 x 64, whole call (us): 64 x 8192 x 1024 11.6 / 16.9, 128 x 8192 x 1024 12.2 / 17.3,
+// 256 x 2048 x 512 6.8 / 8.1, 512 x 8192 x 256 16.2 / 19.9; and where there are two to a CU 128 x 8192 x 2048 20.0 / 16.8.
+constexpr int64_t kCus = 256;
 int launch_product(ProductArgs a, hipStream_t stream) {
   a.out_wide = reinterpret_cast<uintptr_t>(a.out) % 16 == 0 && a.n_out * dtype_size(a.out_dtype) % 16 == 0;
   const int64_t per_group = a.offsets ? ceil_div(a.rows, a.groups) : a.rows;
@@ -741,9 +745,10 @@ int launch_product(ProductArgs a, hipStream_t stream) {
     if (std::min<int64_t>(a.rows, a.rows / 16 + a.groups) * ceil_div(a.n_out, 16) >= 1024) return launch_skinny<1, 2>(a, stream);
     return launch_skinny<1, 4>(a, stream);
   }
+  if ((ceil_div(a.rows, 32) + (a.offsets ? a.groups : 0)) * ceil_div(a.n_out, 16) <= kCus) return launch_skinny<2, 8>(a, stream);
   if (a.offsets == nullptr && a.rows <= 32) return launch_skinny<2, 4>(a, stream);
-  if (per_group >= 256 && tiles(256) >= 256) return launch_tile<2, 4, 4, 2, 2>(a, stream);
-  if ((a.offsets || a.rows >= 96) && tiles(128) >= 256) return launch_tile<2, 4, 2, 1, 2>(a, stream);
+  if (per_group >= 256 && tiles(256) >= kCus) return launch_tile<2, 4, 4, 2, 2>(a, stream);
+  if ((a.offsets || a.rows >= 96) && tiles(128) >= kCus) return launch_tile<2, 4, 2, 1, 2>(a, stream);
   return launch_tile<2, 2, 1, 1, 4>(a, stream);
 }
 

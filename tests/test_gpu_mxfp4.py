@@ -176,6 +176,48 @@ def test_generic_activation_in_large_tiles(amd, oracle):
         assert np.abs(got - np.tanh(before)).max() <= 1e-5
 
 
+@pytest.mark.parametrize('rows, k, n', [(33, 8200, 2500), (64, 1000, 2048), (64, 1000, 2049), (90, 300, 1380), (512, 2080, 256), (512, 100, 260), (700, 32, 200)])
+def test_dense_of_a_middling_size(amd, rows, k, n):
+    """Some tens to some hundreds of rows, on both sides of the size where the form of 32 rows x 16 columns no longer has a compute unit for
+    each of its workgroups; long rows, ragged edges, an activation of its own, and a row and a column of NaN."""
+    rng = np.random.default_rng(rows + n)
+    x, w = _features(rng, (rows, k), torch.bfloat16), _features(rng, (n, k), torch.float32) * 0.05
+    bias = torch.as_tensor(rng.standard_normal(n), dtype=torch.float32).cuda()
+    w4 = amd.mxfp4_quantize(w)
+    x64, w64 = _plain(amd.mxfp4_quantize(x)), _plain(w4)
+    _check_product(amd.mxfp4_dense(x, w4, bias, 'relu'), x64, w64, bias.double().cpu().numpy(), True, torch.bfloat16)
+    clean = amd.mxfp4_dense(x, w4, None, None, torch.float32)
+    _check_product(clean, x64, w64, None, False, torch.float32)
+    # both evaluate tanh of the same float32 sum: the function's own error, as in the other layers
+    tanh = amd.mxfp4_dense(x, w4, None, 'tanh', torch.float32).double().cpu().numpy()
+    assert np.abs(tanh - np.tanh(clean.double().cpu().numpy())).max() <= 1e-5
+    x[rows - 1, k - 1] = float('nan')
+    w[n - 1, 0] = float('inf')
+    got = amd.mxfp4_dense(x, amd.mxfp4_quantize(w), None, None, torch.float32)
+    assert torch.isnan(got[rows - 1]).all() and torch.isnan(got[:, n - 1]).all()
+    assert torch.equal(got[:rows - 1, :n - 1], clean[:rows - 1, :n - 1])
+
+
+@pytest.mark.parametrize('t, top_k, e, k, n', [(60, 2, 5, 1500, 208), (150, 1, 4, 2080, 130), (100, 3, 9, 33, 64)])
+def test_expert_dense_of_a_middling_size(amd, t, top_k, e, k, n):
+    """Ten to sixty rows per expert and few columns, one expert empty: tiles of 32 rows that end inside an expert."""
+    rng = np.random.default_rng(t)
+    index = rng.integers(-1, e, (t, top_k)).astype(np.int32)
+    index[index == 1] = e - 1
+    plan = amd.expert_plan(torch.as_tensor(index).cuda(), e)
+    x = _features(rng, (t, k), torch.float16)
+    w4 = amd.mxfp4_quantize(_features(rng, (e, n, k), torch.float32))
+    bias = torch.as_tensor(rng.standard_normal((e, n)), dtype=torch.float32).cuda()
+    q = R.dispatch(_plain(amd.mxfp4_quantize(x)), plan.slot.cpu().numpy())
+    offsets = plan.offsets.cpu().numpy()
+    got = amd.mxfp4_expert_dense(x, w4, plan, bias, 'relu')
+    for i in range(e):
+        lo, hi = offsets[i], offsets[i + 1]
+        if lo < hi:
+            _check_product(got[lo:hi], q[lo:hi], _plain3(w4)[i], bias[i].double().cpu().numpy(), True, torch.float16)
+    assert not got[offsets[e]:].any()
+
+
 @pytest.mark.parametrize('t, top_k, e, k, n', [(3000, 2, 3, 160, 3000), (1700, 1, 6, 40, 8200), (700, 3, 40, 64, 4104)])
 def test_expert_dense_in_every_tile_size(amd, t, top_k, e, k, n):
     """Uneven experts, one of them empty and one of a single row, in tiles of 256, 128 and 64 rows."""
