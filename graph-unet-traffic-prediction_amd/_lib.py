@@ -233,12 +233,14 @@ def current_stream(device):
 _raw_stream = (getattr(torch._C, '_cuda_getCurrentRawStream', None)
                or (lambda index: torch.cuda.current_stream(index).cuda_stream))
 
+_current_device = getattr(torch._C, '_cuda_getDevice', None) or torch.cuda.current_device
+
 
 def launch(fn_name, device, *args):
     """call(fn_name, *args, stream) on the current stream of `device`, whichever device is current (the null stream belongs
     to the current one).  Pointers are plain addresses: for calls whose kernels take a few microseconds."""
     index = device.index
-    if torch.cuda.current_device() == index:
+    if _current_device() == index:
         status = getattr(lib, fn_name)(*args, _raw_stream(index))
     else:
         with torch.cuda.device(index):

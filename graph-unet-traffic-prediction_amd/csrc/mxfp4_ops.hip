@@ -47,41 +47,85 @@ struct QuantArgs {
 
 // Eight elements of a row from column `col` on (columns past k read as 0): the lane's share of its block.
 template <typename T, bool VEC>
-__device__ __forceinline__ void load_eight(const T* row, int col, int k, float (&v)[8]) {
+__device__ __forceinline__ Pack<T, 8> load_eight(const T* row, int col, int k) {
+  Pack<T, 8> v;
   if (col + 8 <= k) {
     constexpr int kPer = 16 / sizeof(T);
 #pragma unroll
-    for (int p = 0; p < 8 / kPer; ++p) {
+    for (int p = 0; p < 8; p += kPer) {
       Pack<T, kPer> q;
       if (VEC)
-        q = load_pack<T, kPer>(row + col + p * kPer);
+        q = load_pack<T, kPer>(row + col + p);
       else
-        __builtin_memcpy(&q, row + col + p * kPer, sizeof(q));     // an unaligned load
+        __builtin_memcpy(&q, row + col + p, sizeof(q));     // an unaligned load
 #pragma unroll
-      for (int c = 0; c < kPer; ++c) v[p * kPer + c] = to_f32(q.v[c]);
+      for (int c = 0; c < kPer; ++c) v.v[p + c] = q.v[c];
     }
   } else {
 #pragma unroll
-    for (int c = 0; c < 8; ++c) v[c] = col + c < k ? to_f32(row[col + c]) : 0.0f;
+    for (int c = 0; c < 8; ++c) v.v[c] = col + c < k ? row[col + c] : static_cast<T>(0.0f);
   }
+  return v;
 }
 
-// Four neighbouring lanes hold a block, eight elements each: returns the lane's eight codes and the block's scale byte.
-__device__ __forceinline__ uint32_t quantize_eight(const float (&v)[8], uint32_t* byte) {
+// The value of a neighbour among four lanes: CTRL 0xB1 exchanges lanes 0, 1 and 2, 3, CTRL 0x4E the two pairs.
+template <int CTRL>
+__device__ __forceinline__ uint32_t of_four(uint32_t v) {
+  return static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), CTRL, 0xF, 0xF, true));
+}
+
+// Four neighbouring lanes hold a block, eight elements each: returns the lane's eight codes and the block's scale byte.  Two-byte types stay as
+// they are, two to a register: the instruction converts them from that (both types exactly, as the float32 form does).
+template <typename T>
+__device__ __forceinline__ uint32_t quantize_eight(const Pack<T, 8>& v, uint32_t* byte) {
   // magnitudes as integers: NaN sorts above infinity, infinity above every number
   uint32_t top = 0;
+  if constexpr (sizeof(T) == 4) {
 #pragma unroll
-  for (int c = 0; c < 8; ++c) top = max(top, __float_as_uint(v[c]) & 0x7FFFFFFFu);
-  top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 1)));
-  top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 2)));
-  const int exponent = static_cast<int>(top >> 23);
+    for (int c = 0; c < 8; ++c) top = max(top, __float_as_uint(v.v[c]) & 0x7FFFFFFFu);
+  } else {
+    typedef uint16_t Two __attribute__((ext_vector_type(2)));
+    const u32x4 w = __builtin_bit_cast(u32x4, v);
+    Two most = {0, 0};
+#pragma unroll
+    for (int c = 0; c < 4; ++c) most = __builtin_elementwise_max(most, __builtin_bit_cast(Two, w[c] & 0x7FFF7FFFu));
+    top = max(most[0], most[1]);
+  }
+  top = max(top, of_four<0xB1>(top));
+  top = max(top, of_four<0x4E>(top));
+  int exponent;      // of the float32 value
+  if constexpr (sizeof(T) == 4)
+    exponent = static_cast<int>(top >> 23);
+  else if constexpr (std::is_same<T, __bf16>::value)
+    exponent = static_cast<int>(top >> 7);
+  else
+    exponent = top >= 0x7C00u ? 255 : static_cast<int>(__float_as_uint(to_f32(__builtin_bit_cast(_Float16, static_cast<uint16_t>(top)))) >> 23);
   *byte = exponent == 255 ? 255u : static_cast<uint32_t>(max(exponent - 2, 0));
   if (exponent == 255) return 0;
   const float s = scale_value(*byte);
-  uint32_t word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0u, v[0], v[1], s, 0);
-  word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, v[2], v[3], s, 1);
-  word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, v[4], v[5], s, 2);
-  return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, v[6], v[7], s, 3);
+  uint32_t word = 0;
+  if constexpr (sizeof(T) == 4) {
+    word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, v.v[0], v.v[1], s, 0);
+    word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, v.v[2], v.v[3], s, 1);
+    word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, v.v[4], v.v[5], s, 2);
+    return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, v.v[6], v.v[7], s, 3);
+  } else {
+    typedef T Two __attribute__((ext_vector_type(2)));
+    const u32x4 w = __builtin_bit_cast(u32x4, v);
+    const uint32_t w0 = w[0], w1 = w[1], w2 = w[2], w3 = w[3];      // a bit cast of a vector's element itself takes element 0
+    const Two a = __builtin_bit_cast(Two, w0), b = __builtin_bit_cast(Two, w1), c = __builtin_bit_cast(Two, w2), d = __builtin_bit_cast(Two, w3);
+    if constexpr (std::is_same<T, __bf16>::value) {
+      word = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(word, a, s, 0);
+      word = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(word, b, s, 1);
+      word = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(word, c, s, 2);
+      return __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(word, d, s, 3);
+    } else {
+      word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(word, a, s, 0);
+      word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(word, b, s, 1);
+      word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(word, c, s, 2);
+      return __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(word, d, s, 3);
+    }
+  }
 }
 
 // Four lanes share a block: its amax takes two exchanges inside a group of four lanes, the codes of a lane are one dword.  HBM-bound: x
@@ -101,10 +145,8 @@ __global__ __launch_bounds__(kThreads) void k_mxfp4_quantize(QuantArgs a, const 
     const int64_t row = i / parts;
     const int part = static_cast<int>(i - row * parts);
     const int block = part >> 2;
-    float v[8];
-    load_eight<T, VEC>(x + row * a.k, part * 8, a.k, v);
     uint32_t byte;
-    const uint32_t word = quantize_eight(v, &byte);
+    const uint32_t word = quantize_eight(load_eight<T, VEC>(x + row * a.k, part * 8, a.k), &byte);
     const int copies = a.slot ? a.top_k : 1;
     for (int j = 0; j < copies; ++j) {
       int64_t r = row;
@@ -589,10 +631,8 @@ __global__ __launch_bounds__(64 * NW) void k_mxfp4_skinny(ProductArgs a) {
       const int row_parts = a.blocks * 4;
       for (int i = threadIdx.x; i < t.rows * row_parts; i += 64 * NW) {
         const int row = i / row_parts, part = i - row * row_parts, block = part >> 2;
-        float v[8];
-        load_eight<XT, VEC>(static_cast<const XT*>(a.x) + (t.row0 + row) * a.k, part * 8, a.k, v);
         uint32_t byte;
-        const uint32_t word = quantize_eight(v, &byte);
+        const uint32_t word = quantize_eight(load_eight<XT, VEC>(static_cast<const XT*>(a.x) + (t.row0 + row) * a.k, part * 8, a.k), &byte);
         *reinterpret_cast<uint32_t*>(raw_smem + row * stride + part * 4) = word;
         char* const s8 = raw_scales + row * a.tiles * 8;
         if ((part & 3) == 0) s8[block] = static_cast<char>(byte);
@@ -672,6 +712,8 @@ int launch_quantize(const void* x, int32_t dtype, int64_t groups, int64_t rows, 
   return GUNET_OK;
 }
 
+constexpr int64_t kCus = 256;     // compute units
+
 template <int WM, int WN, int FM, int FN, int STAGES>
 int launch_tile(ProductArgs a, hipStream_t stream) {
   using S = TileShape<WM, WN, FM, FN, STAGES>;
@@ -700,17 +742,22 @@ int launch_skinny(ProductArgs a, hipStream_t stream, size_t lds = 0) {
   return GUNET_OK;
 }
 
-// Whether the product of one group quantises x on its way.  Every workgroup does all of it, so it
-// pays for little x only.  Whole call, one launch against two (us): 1 x 4096 x 4096 4.5 / 5.7, 1 x 8192 x 8192 9.4 / 10.3, 2 x 4096 x 4096
-// 5.4 / 6.0, 16 x 1024 x 8192 6.6 / 6.0, 4 x 4096 x 4096 7.3 / 6.2, 16 x 2048 x 2048 10.2 / 5.8.
-constexpr int64_t kRawElements = 8192;
+// Whether the product of one group quantises x on its way.  Every workgroup does all of it, so it pays for little x only; it saves a launch, of
+// which the host makes one in 3.5 us.  Whole bf16 call, one launch against two, in a captured graph (us): 1 x 4096 x 4096 4.8 / 6.6,
+// 2 x 8192 x 8192 13.0 / 13.7, 4 x 4096 x 4096 5.7 / 7.1, 16 x 1024 x 8192 5.9 / 6.5, 16 x 1024 x 1024 3.9 / 5.0; called one by one 7.7 / 11.9.  At
+// twice as much x 4 x 8192 x 4096 8.8 / 9.0, 16 x 2048 x 8192 8.9 / 7.5.
+constexpr int64_t kRawElements = 16384;
 bool raw_form(int64_t rows, int64_t k) { return rows <= 16 && rows * k <= kRawElements; }
 
+// Sixteen waves quantise faster than eight, where they are a CU's only ones: 4 x 4096 x 1024 4.4 us against 4.8, 1 x 8192 x 1024 5.2 against 5.5,
+// 1 x 4096 x 4096 4.8 both; with two workgroups to a CU 1 x 8192 x 8192 12.8 against 11.9, 16 x 1024 x 8192 7.0 against 5.9.  (Four waves: 4 x 4096 x 1024 6.0.)
 template <typename XT>
 int launch_raw(const ProductArgs& a, hipStream_t stream) {
   const size_t lds = static_cast<size_t>(a.rows) * (a.blocks * 16 + a.tiles * 8);
   const bool vec = reinterpret_cast<uintptr_t>(a.x) % 16 == 0 && a.k * sizeof(XT) % 16 == 0;
-  return vec ? launch_skinny<1, 4, XT, true>(a, stream, lds) : launch_skinny<1, 4, XT, false>(a, stream, lds);
+  if (a.rows * a.k > 4096 && ceil_div(a.n_out, 16) <= kCus)
+    return vec ? launch_skinny<1, 16, XT, true>(a, stream, lds) : launch_skinny<1, 16, XT, false>(a, stream, lds);
+  return vec ? launch_skinny<1, 8, XT, true>(a, stream, lds) : launch_skinny<1, 8, XT, false>(a, stream, lds);
 }
 
 // Which form.  Rows per group decide how many rows a tile can fill, the number of tiles whether they fill the chip (256 CUs).
@@ -734,7 +781,6 @@ int launch_raw(const ProductArgs& a, hipStream_t stream) {
 // A CU takes in about 50 bytes a ns whatever the form, so a product of few tiles gains by smaller ones as long as each has a CU of its
 // own: 32 rows x 16 columns, eight waves sharing K, against 64 x 64, whole call (us): 64 x 8192 x 1024 11.6 / 16.9, 128 x 8192 x 1024 12.2 / 17.3,
 // 256 x 2048 x 512 6.8 / 8.1, 512 x 8192 x 256 16.2 / 19.9; and where there are two to a CU 128 x 8192 x 2048 20.0 / 16.8.
-constexpr int64_t kCus = 256;
 int launch_product(ProductArgs a, hipStream_t stream) {
   a.out_wide = reinterpret_cast<uintptr_t>(a.out) % 16 == 0 && a.n_out * dtype_size(a.out_dtype) % 16 == 0;
   const int64_t per_group = a.offsets ? ceil_div(a.rows, a.groups) : a.rows;

@@ -69,7 +69,7 @@ def expert_plan(expert_index, n_experts):
     dev = index.device
     offsets = index.new_empty(max(0, min(n_experts, _lib.MAX_EXPERTS)) + 1)       # the library refuses other numbers
     order = index.new_empty(t * k)
-    slot = index.new_empty((t, k))
+    slot = torch.empty_like(index)
     nbytes = _lib.lib.gunet_expert_sort_workspace_bytes(t, k, n_experts)
     scratch = index.new_empty(nbytes // 4) if nbytes else None
     launch('gunet_expert_sort', dev, index.data_ptr(), t, k, n_experts, offsets.data_ptr(), order.data_ptr(), slot.data_ptr(),

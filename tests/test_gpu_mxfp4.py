@@ -102,6 +102,34 @@ def test_quantize_ties_ends_and_special_values(amd):
     assert np.array_equal(np.signbit(back[-4]), np.ones(32, bool))
 
 
+@pytest.mark.parametrize('dtype, mantissa', [(torch.bfloat16, 7), (torch.float16, 10)], ids=str)
+def test_quantize_two_byte_values_at_every_exponent(amd, dtype, mantissa):
+    """Blocks with every exponent as their largest value's (subnormals too), filled with the numbers of either sign down to 2^-8 of it: every
+    rounding there is, in both packed halves.  And infinities and NaN in every place of a block."""
+    every = torch.arange(1 << 16, dtype=torch.int32).to(torch.int16).view(dtype)
+    every = every[torch.isfinite(every)]
+    size = every.double().abs()
+    blocks = []
+    for exponent in range((1 << (15 - mantissa)) - 1):
+        for rest in (0, 1, (1 << mantissa) - 1):
+            top = torch.tensor([exponent << mantissa | rest], dtype=torch.int16).view(dtype)
+            fill = every[(size <= top.double()) & (size >= top.double() * 2.0 ** -8)]
+            fill = fill[:fill.numel() // 31 * 31].view(-1, 31)
+            blocks.append(torch.cat([top.expand(fill.shape[0], 1), fill], 1))
+            blocks.append(torch.cat([fill, top.expand(fill.shape[0], 1)], 1))
+    x = torch.cat(blocks).contiguous()
+    assert x.shape[0] > 1 << 16
+    code, scales = R.quantize(x.double().numpy())
+    t = amd.mxfp4_quantize(x.cuda())
+    assert np.array_equal(t.codes[0].cpu().numpy(), R.pack(code))
+    assert np.array_equal(t.scales[0, 0, :, 0].cpu().numpy(), scales[:, 0])
+    x = torch.ones((96, 64), dtype=dtype)
+    for i, bad in enumerate((float('inf'), -float('inf'), float('nan'))):
+        x[32 * i + torch.arange(32), torch.arange(32)] = bad
+    back = amd.mxfp4_dequantize(amd.mxfp4_quantize(x.cuda())).cpu()
+    assert torch.isnan(back[:, :32]).all() and (back[:, 32:] == 1).all()
+
+
 def test_quantize_stacks_strides_and_unaligned(amd):
     x = _features(np.random.default_rng(1), (3, 10, 96), torch.bfloat16)
     t = amd.mxfp4_quantize(x)
@@ -174,6 +202,27 @@ def test_generic_activation_in_large_tiles(amd, oracle):
         before = amd.mxfp4_dense(x, w).double().cpu().numpy()
         got = amd.mxfp4_dense(x, w, None, 'tanh').double().cpu().numpy()
         assert np.abs(got - np.tanh(before)).max() <= 1e-5
+
+
+@pytest.mark.parametrize('dtype', TYPES, ids=str)
+@pytest.mark.parametrize('rows, k, n', [(1, 16384, 33), (16, 1024, 100), (16, 1024, 4100), (4, 4095, 50), (3, 4100, 4112), (15, 1090, 17), (16, 1025, 40), (16, 1, 3), (1, 4097, 1)])
+def test_dense_of_a_few_rows(amd, dtype, rows, k, n):
+    """Both sides of the sizes up to which x is quantised inside the product, and of those that decide how many waves share that."""
+    rng = np.random.default_rng(rows + k)
+    x, w4 = _features(rng, (rows, k), dtype), amd.mxfp4_quantize(_features(rng, (n, k), torch.float32))
+    bias = torch.as_tensor(rng.standard_normal(n), dtype=torch.float32).cuda()
+    x64, w64 = _plain(amd.mxfp4_quantize(x)), _plain(w4)
+    _check_product(amd.mxfp4_dense(x, w4, bias, 'relu', torch.float32), x64, w64, bias.double().cpu().numpy(), True, torch.float32)
+    got = amd.mxfp4_dense(x, w4, None, None, torch.float32)
+    _check_product(got, x64, w64, None, False, torch.float32)
+    odd = torch.zeros(rows * k + 1, dtype=dtype, device='cuda')[1:].view(rows, k)       # rows that start on no 16 bytes
+    odd.copy_(x)
+    assert torch.equal(amd.mxfp4_dense(odd, w4, None, None, torch.float32), got)
+    tanh = amd.mxfp4_dense(x, w4, None, 'tanh', torch.float32).double().cpu().numpy()
+    assert np.abs(tanh - np.tanh(got.double().cpu().numpy())).max() <= 1e-5             # the same float32 sum on both sides
+    x[rows - 1, k - 1] = float('nan')
+    bad = amd.mxfp4_dense(x, w4, None, None, torch.float32)
+    assert torch.isnan(bad[rows - 1]).all() and torch.equal(bad[:rows - 1], got[:rows - 1])
 
 
 @pytest.mark.parametrize('rows, k, n', [(33, 8200, 2500), (64, 1000, 2048), (64, 1000, 2049), (90, 300, 1380), (512, 2080, 256), (512, 100, 260), (700, 32, 200)])
