@@ -212,8 +212,9 @@ __global__ __launch_bounds__(kThreads) void k_mxfp4_dequantize(int64_t rows, int
 
 // out[r][n] = act(sum_k x[r][k] w[g][n][k] + bias[g][n]) for the rows of group g.
 struct ProductArgs {
-  const void* x;              // [rows][k], for the form that quantises on the way
-  int32_t k;
+  const void* x;              // for the form that quantises on the way: [rows][k], or with slot [rows / top_k][k]
+  const int32_t* slot;        // [rows] or null: row r is a copy of the one whose choice has slot r
+  int32_t k, top_k;
   const uint8_t* x_codes;     // [rows][blocks * 16]
   const uint8_t* x_scales;    // [tiles][rows][8]
   const uint8_t* w_codes;     // [groups][n_out][blocks * 16]
@@ -290,6 +291,14 @@ __device__ __forceinline__ bool find_row_tile(const ProductArgs& a, int size, in
     done += __shfl(upto, 63);
   }
   return false;
+}
+
+// The row of x that row r is a copy of; there are 16 slots at most.
+__device__ __forceinline__ int64_t source_row(const ProductArgs& a, int64_t r) {
+  if (a.slot == nullptr) return r;
+  int at = 0;
+  for (int j = 0; j < static_cast<int>(a.rows); ++j) at = a.slot[j] == r ? j : at;
+  return at / a.top_k;
 }
 
 __device__ __forceinline__ void store_out(void* out, int dtype, int64_t at, float v) {
@@ -559,8 +568,8 @@ __device__ __forceinline__ v4f mfma16_fp4(u32x4 a, u32x4 b, v4f c, int step, int
 // share the K axis out among them in turns of 512 columns (v_mfma_scale_f32_16x16x128: quarter-wave q takes blocks 4 q + s of 16, s = 0..3, its
 // scales again one dword), straight from memory to registers with the next turn's loads on their way, and add their parts through LDS in
 // wave order.  No barrier inside the K loop.
-// XT = void: x comes quantised.  Else x is [rows][k] of that type, and every workgroup quantises its rows into LDS while its first weights
-// are on their way, which saves the launch (and the time) of doing it before; one group, MF = 1.
+// XT = void: x comes quantised.  Else x is of that type, and every workgroup quantises its rows (16 at most in all, MF = 1) into LDS while its
+// first weights are on their way, which saves the launch (and the time) of doing it before.
 template <int MF, int NW, typename XT, bool VEC, bool ANY_ACT>
 __global__ __launch_bounds__(64 * NW) void k_mxfp4_skinny(ProductArgs a) {
   constexpr bool kRaw = !std::is_same<XT, void>::value;
@@ -632,7 +641,7 @@ __global__ __launch_bounds__(64 * NW) void k_mxfp4_skinny(ProductArgs a) {
       for (int i = threadIdx.x; i < t.rows * row_parts; i += 64 * NW) {
         const int row = i / row_parts, part = i - row * row_parts, block = part >> 2;
         uint32_t byte;
-        const uint32_t word = quantize_eight(load_eight<XT, VEC>(static_cast<const XT*>(a.x) + (t.row0 + row) * a.k, part * 8, a.k), &byte);
+        const uint32_t word = quantize_eight(load_eight<XT, VEC>(static_cast<const XT*>(a.x) + source_row(a, t.row0 + row) * a.k, part * 8, a.k), &byte);
         *reinterpret_cast<uint32_t*>(raw_smem + row * stride + part * 4) = word;
         char* const s8 = raw_scales + row * a.tiles * 8;
         if ((part & 3) == 0) s8[block] = static_cast<char>(byte);
@@ -742,22 +751,33 @@ int launch_skinny(ProductArgs a, hipStream_t stream, size_t lds = 0) {
   return GUNET_OK;
 }
 
-// Whether the product of one group quantises x on its way.  Every workgroup does all of it, so it pays for little x only; it saves a launch, of
-// which the host makes one in 3.5 us.  Whole bf16 call, one launch against two, in a captured graph (us): 1 x 4096 x 4096 4.8 / 6.6,
-// 2 x 8192 x 8192 13.0 / 13.7, 4 x 4096 x 4096 5.7 / 7.1, 16 x 1024 x 8192 5.9 / 6.5, 16 x 1024 x 1024 3.9 / 5.0; called one by one 7.7 / 11.9.  At
-// twice as much x 4 x 8192 x 4096 8.8 / 9.0, 16 x 2048 x 8192 8.9 / 7.5.
+// Whether the product quantises x on its way.  Every workgroup does all of it (of its expert's rows), so it pays for little x only; it saves a launch,
+// of which the host makes one in 3.5 us.  Whole bf16 call, one launch against two, in a captured graph (us): 1 x 4096 x 4096 4.8 / 6.6,
+// 2 x 8192 x 8192 13.0 / 13.7, 4 x 4096 x 4096 5.7 / 7.1, 16 x 1024 x 8192 5.9 / 6.5, 16 x 1024 x 1024 3.9 / 5.0; 1 token x 2 of 8 experts 2048 -> 4096
+// 4.3 / 7.1, 4 x 4 of 32 1024 -> 2048 8.2 / 8.5; called one by one 7.7 / 11.9, experts 8.7 / 12.0.  At twice as much x
+// 4 x 8192 x 4096 8.8 / 9.0, 16 x 2048 x 8192 8.9 / 7.5; 4 x 4 of 16 experts 2048 -> 4096 15.9 / 14.8.
 constexpr int64_t kRawElements = 16384;
 bool raw_form(int64_t rows, int64_t k) { return rows <= 16 && rows * k <= kRawElements; }
 
-// Sixteen waves quantise faster than eight, where they are a CU's only ones: 4 x 4096 x 1024 4.4 us against 4.8, 1 x 8192 x 1024 5.2 against 5.5,
-// 1 x 4096 x 4096 4.8 both; with two workgroups to a CU 1 x 8192 x 8192 12.8 against 11.9, 16 x 1024 x 8192 7.0 against 5.9.  (Four waves: 4 x 4096 x 1024 6.0.)
-template <typename XT>
+// One group: sixteen waves quantise faster than eight, where they are a CU's only ones: 4 x 4096 x 1024 4.4 us against 4.8, 1 x 8192 x 1024 5.2 against
+// 5.5, 1 x 4096 x 4096 4.8 both; with two workgroups to a CU 1 x 8192 x 8192 12.8 against 11.9, 16 x 1024 x 8192 7.0 against 5.9.  (Four waves: 4 x 4096 x 1024 6.0.)
+// Experts, of which most have a row or two here: four waves, 1 token x 4 of 32 experts 2048 -> 4096 6.6 us against 8.3 with eight, and eight where
+// few workgroups have long rows, 1 x 2 of 8 4096 -> 4096 6.4 against 7.3; in two launches 9.1 and 8.5.
+template <typename XT, bool VEC>
 int launch_raw(const ProductArgs& a, hipStream_t stream) {
   const size_t lds = static_cast<size_t>(a.rows) * (a.blocks * 16 + a.tiles * 8);
+  const int64_t col_tiles = ceil_div(a.n_out, 16);
+  if (a.offsets) {
+    if (a.k > 2048 && std::min<int64_t>(a.rows, a.groups + 1) * col_tiles <= 2 * kCus) return launch_skinny<1, 8, XT, VEC>(a, stream, lds);
+    return launch_skinny<1, 4, XT, VEC>(a, stream, lds);
+  }
+  if (a.rows * a.k > 4096 && col_tiles <= kCus) return launch_skinny<1, 16, XT, VEC>(a, stream, lds);
+  return launch_skinny<1, 8, XT, VEC>(a, stream, lds);
+}
+template <typename XT>
+int launch_raw(const ProductArgs& a, hipStream_t stream) {
   const bool vec = reinterpret_cast<uintptr_t>(a.x) % 16 == 0 && a.k * sizeof(XT) % 16 == 0;
-  if (a.rows * a.k > 4096 && ceil_div(a.n_out, 16) <= kCus)
-    return vec ? launch_skinny<1, 16, XT, true>(a, stream, lds) : launch_skinny<1, 16, XT, false>(a, stream, lds);
-  return vec ? launch_skinny<1, 8, XT, true>(a, stream, lds) : launch_skinny<1, 8, XT, false>(a, stream, lds);
+  return vec ? launch_raw<XT, true>(a, stream) : launch_raw<XT, false>(a, stream);
 }
 
 // Which form.  Rows per group decide how many rows a tile can fill, the number of tiles whether they fill the chip (256 CUs).
@@ -817,7 +837,9 @@ int run_dense(const char* fn, const void* x, int32_t dtype, int64_t x_rows, int6
                 "%s: x or out is not aligned to its type", fn);
   ProductArgs a = {};
   a.x = x;
+  a.slot = slot;
   a.k = k;
+  a.top_k = top_k;
   a.w_codes = w_codes;
   a.w_scales = w_scales;
   a.bias = bias;
@@ -830,17 +852,18 @@ int run_dense(const char* fn, const void* x, int32_t dtype, int64_t x_rows, int6
   a.groups = groups;
   a.act = activation;
   a.out_dtype = out_dtype;
-  if (offsets == nullptr && raw_form(rows, k)) {
+  const bool raw = raw_form(rows, k);
+  const int64_t codes = align256(code_bytes(rows, k)), need = raw && offsets == nullptr ? 0 : codes + scale_bytes(rows, k);
+  if (need > 0 && (workspace == nullptr || workspace_bytes < static_cast<size_t>(need))) {
+    set_error("%s: workspace of %zu bytes, %lld are needed", fn, workspace ? workspace_bytes : size_t{0}, static_cast<long long>(need));
+    return GUNET_ERR_WORKSPACE;
+  }
+  GUNET_REQUIRE(need == 0 || reinterpret_cast<uintptr_t>(workspace) % 16 == 0, "%s: workspace is not 16-byte aligned", fn);
+  if (raw) {
     if (dtype == GUNET_DTYPE_F32) return launch_raw<float>(a, stream);
     if (dtype == GUNET_DTYPE_BF16) return launch_raw<__bf16>(a, stream);
     return launch_raw<_Float16>(a, stream);
   }
-  const int64_t codes = align256(code_bytes(rows, k)), need = codes + scale_bytes(rows, k);
-  if (workspace == nullptr || workspace_bytes < static_cast<size_t>(need)) {
-    set_error("%s: workspace of %zu bytes, %lld are needed", fn, workspace ? workspace_bytes : size_t{0}, static_cast<long long>(need));
-    return GUNET_ERR_WORKSPACE;
-  }
-  GUNET_REQUIRE(reinterpret_cast<uintptr_t>(workspace) % 16 == 0, "%s: workspace is not 16-byte aligned", fn);
   uint8_t* const x_codes = static_cast<uint8_t*>(workspace);
   GUNET_TRY(launch_quantize(x, dtype, 1, x_rows, rows, k, top_k, slot, x_codes, x_codes + codes, stream));
   a.x_codes = x_codes;

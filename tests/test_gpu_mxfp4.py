@@ -247,6 +247,35 @@ def test_dense_of_a_middling_size(amd, rows, k, n):
     assert torch.equal(got[:rows - 1, :n - 1], clean[:rows - 1, :n - 1])
 
 
+@pytest.mark.parametrize('dtype', TYPES, ids=str)
+@pytest.mark.parametrize('t, top_k, e, k, n', [(1, 1, 3, 2049, 40), (1, 2, 8, 8192, 48), (1, 16, 20, 100, 33), (4, 4, 6, 1024, 130), (4, 4, 6, 1025, 130), (2, 3, 8, 2500, 48),
+                                               (16, 1, 2, 1000, 16), (17, 1, 3, 64, 16), (3, 5, 1, 33, 257)])
+def test_expert_dense_of_a_few_rows(amd, dtype, t, top_k, e, k, n):
+    """Both sides of the sizes up to which the tokens are quantised inside the experts' product; a dropped choice, an expert named twice."""
+    rng = np.random.default_rng(t * k + top_k)
+    index = rng.integers(0, e, (t, top_k)).astype(np.int32)
+    if t * top_k > 2:
+        index[t // 2, top_k - 1] = -1
+    plan = amd.expert_plan(torch.as_tensor(index).cuda(), e)
+    x, w4 = _features(rng, (t, k), dtype), amd.mxfp4_quantize(_features(rng, (e, n, k), torch.float32))
+    bias = torch.as_tensor(rng.standard_normal((e, n)), dtype=torch.float32).cuda()
+    q, w64 = R.dispatch(_plain(amd.mxfp4_quantize(x)), plan.slot.cpu().numpy()), _plain3(w4)
+    offsets, order = plan.offsets.cpu().numpy(), plan.order.cpu().numpy()
+    got = amd.mxfp4_expert_dense(x, w4, plan, bias, 'relu', torch.float32)
+    for i in range(e):
+        lo, hi = offsets[i], offsets[i + 1]
+        _check_product(got[lo:hi], q[lo:hi], w64[i], bias[i].double().cpu().numpy(), True, torch.float32)
+    assert not got[offsets[e]:].any()
+    ready = amd.expert_dispatch(x, plan)
+    assert torch.equal(amd.mxfp4_expert_dense(ready, w4, plan, bias, 'relu', torch.float32, sorted_rows=True), got)
+    odd = torch.zeros(t * k + 1, dtype=dtype, device='cuda')[1:].view(t, k)             # rows that start on no 16 bytes
+    odd.copy_(x)
+    assert torch.equal(amd.mxfp4_expert_dense(odd, w4, plan, bias, 'relu', torch.float32), got)
+    x[t - 1, k - 1] = float('nan')
+    bad = torch.isnan(amd.mxfp4_expert_dense(x, w4, plan)).all(1).cpu().numpy()
+    assert np.array_equal(bad, (order >= 0) & (order // top_k == t - 1))
+
+
 @pytest.mark.parametrize('t, top_k, e, k, n', [(60, 2, 5, 1500, 208), (150, 1, 4, 2080, 130), (100, 3, 9, 33, 64)])
 def test_expert_dense_of_a_middling_size(amd, t, top_k, e, k, n):
     """Ten to sixty rows per expert and few columns, one expert empty: tiles of 32 rows that end inside an expert."""
