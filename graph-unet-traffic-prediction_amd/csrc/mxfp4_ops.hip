@@ -792,12 +792,22 @@ int launch_raw(const ProductArgs& a, hipStream_t stream) {
 //   48332 x 256 x 256                              16.4       10.5         9.9
 //   4096 x 4096 x 4096                             79.8       48.5        37.7
 //   8192 x 8192 x 8192                              540        326         258
-// and 32 experts 2048 -> 4096 with their quantisation, by average rows per expert:
-//   4                           35.5               39.7       39.3        48.5
-//   8                           42.2               41.4       41.1        49.2
-//   64                           147               57.5       53.9        58.4
-//   128                          269               86.4       62.2        69.1
-//   256                          492                152        102        91.3
+// and experts with their quantisation, by average rows per expert:
+//                           16 columns   32 x 128   64 x 128   64 x 64   128 x 128   256 x 256
+//   32 of 2048 -> 4096:  1        20.1       22.5       20.7      20.4        29.3        41.7
+//                        4        35.4       34.9       39.7      39.7        39.1        48.5
+//                        8        41.8       36.4       40.8      40.7        41.1        49.2
+//                       16        56.4       40.0       43.5      45.1        43.0        51.0
+//                       32        87.3       43.8       44.5      47.5        47.5        52.9
+//                       64         147       57.5       47.6      58.1        53.9        57.9
+//                      128         269       88.6       65.4      86.4        62.7        68.2
+//                      256                    157        107       152         101        91.7
+//   64 of 1024 -> 1024:  3        13.6       12.5       12.7
+//                       16                   16.1       14.0      14.6        14.7
+//                       48                   19.8       15.8                  19.8
+//    8 of 4096 -> 2048, too few tiles of 128 columns to fill the chip:
+//                        4        12.9       13.6       17.5
+//                       32                   14.2       18.0      14.0        19.4
 // A CU takes in about 50 bytes a ns whatever the form, so a product of few tiles gains by smaller ones as long as each has a CU of its
 // own: 32 rows x 16 columns, eight waves sharing K, against 64 x 64, whole call (us): 64 x 8192 x 1024 11.6 / 16.9, 128 x 8192 x 1024 12.2 / 17.3,
 // 256 x 2048 x 512 6.8 / 8.1, 512 x 8192 x 256 16.2 / 19.9; and where there are two to a CU 128 x 8192 x 2048 20.0 / 16.8.
@@ -805,9 +815,15 @@ int launch_product(ProductArgs a, hipStream_t stream) {
   a.out_wide = reinterpret_cast<uintptr_t>(a.out) % 16 == 0 && a.n_out * dtype_size(a.out_dtype) % 16 == 0;
   const int64_t per_group = a.offsets ? ceil_div(a.rows, a.groups) : a.rows;
   const auto tiles = [&](int64_t size) { return (a.rows / size + (a.offsets ? a.groups / 2 : 1)) * ceil_div(a.n_out, size); };
+  const int64_t expert_tiles = a.offsets ? a.groups * ceil_div(a.n_out, 128) : 0;      // if each expert's rows fit one row tile
+  if (expert_tiles >= kCus && per_group >= 2 && per_group <= 96) {
+    // experts have uneven numbers of rows, so 32 rows hold most of them up to an average of 12 only; where there are many tiles to hide in, of 24
+    if (per_group < 12 || (per_group <= 24 && expert_tiles >= 4 * kCus)) return launch_tile<1, 4, 1, 1, 3>(a, stream);
+    return launch_tile<2, 2, 1, 2, 2>(a, stream);
+  }
   if (per_group <= (a.offsets ? 6 : 16)) {
     // two waves a workgroup stream as well as four once there are four workgroups per CU, and leave more of them side by side: 35.5 us
-    // against 41.6 in the experts' first line
+    // against 41.6 for 32 experts of 4 rows each
     if (std::min<int64_t>(a.rows, a.rows / 16 + a.groups) * ceil_div(a.n_out, 16) >= 1024) return launch_skinny<1, 2>(a, stream);
     return launch_skinny<1, 4>(a, stream);
   }

@@ -276,6 +276,34 @@ def test_expert_dense_of_a_few_rows(amd, dtype, t, top_k, e, k, n):
     assert np.array_equal(bad, (order >= 0) & (order // top_k == t - 1))
 
 
+@pytest.mark.parametrize('t, top_k, e, k, n, dtype', [
+    (100, 3, 40, 288, 1000, torch.bfloat16), (90, 3, 40, 520, 1001, torch.float16), (1500, 1, 64, 33, 2050, torch.float32),         # 32 x 128 tiles
+    (500, 2, 64, 100, 1032, torch.float32), (3000, 1, 40, 300, 833, torch.bfloat16), (700, 3, 37, 1030, 904, torch.float16),        # 64 x 128
+    (300, 1, 5, 160, 4100, torch.bfloat16), (700, 2, 5, 64, 4100, torch.float16)], ids=str)                                        # 64 x 64, 128 x 128
+def test_expert_dense_with_some_rows_each(amd, t, top_k, e, k, n, dtype):
+    """Two to three hundred rows per expert on average, very unevenly: experts of no row, of one, of several tiles; dropped choices."""
+    rng = np.random.default_rng(t + n)
+    share = rng.permutation(np.arange(e) ** 2 + 0.0)
+    index = np.where(rng.random((t, top_k)) < 0.05, -1, rng.choice(e, (t, top_k), p=share / share.sum())).astype(np.int32)
+    plan = amd.expert_plan(torch.as_tensor(index).cuda(), e)
+    x, w4 = _features(rng, (t, k), dtype), amd.mxfp4_quantize(_features(rng, (e, n, k), torch.bfloat16))
+    bias = torch.as_tensor(rng.standard_normal((e, n)), dtype=torch.float32).cuda()
+    q, w64 = R.dispatch(_plain(amd.mxfp4_quantize(x)), plan.slot.cpu().numpy()), _plain3(w4)
+    offsets = plan.offsets.cpu().numpy()
+    assert (np.diff(offsets) == 0).any()
+    got = amd.mxfp4_expert_dense(x, w4, plan, bias, 'relu')
+    full = amd.mxfp4_expert_dense(x, w4, plan, None, None, torch.float32)
+    tanh = amd.mxfp4_expert_dense(x, w4, plan, None, 'tanh', torch.float32)
+    for i in range(e):
+        lo, hi = offsets[i], offsets[i + 1]
+        _check_product(got[lo:hi], q[lo:hi], w64[i], bias[i].double().cpu().numpy(), True, dtype)
+        _check_product(full[lo:hi], q[lo:hi], w64[i], None, False, torch.float32)
+    assert (tanh.double() - torch.tanh(full.double())).abs().max() <= 1e-5             # the same float32 sum on both sides
+    assert not got[offsets[e]:].any() and not full[offsets[e]:].any() and not tanh[offsets[e]:].any()
+    ready = amd.expert_dispatch(x, plan)
+    assert torch.equal(amd.mxfp4_expert_dense(ready, w4, plan, bias, 'relu', sorted_rows=True), got)
+
+
 @pytest.mark.parametrize('t, top_k, e, k, n', [(60, 2, 5, 1500, 208), (150, 1, 4, 2080, 130), (100, 3, 9, 33, 64)])
 def test_expert_dense_of_a_middling_size(amd, t, top_k, e, k, n):
     """Ten to sixty rows per expert and few columns, one expert empty: tiles of 32 rows that end inside an expert."""
