@@ -788,10 +788,18 @@ int launch_raw(const ProductArgs& a, hipStream_t stream) {
 //   64 x 4096 x 4096             8.6                7.8       13.3        26.6
 //   256 x 4096 x 4096           26.5                8.9       14.3        27.6
 //   2048 x 8192 x 1024                             18.8       25.1        48.6
-//   1024 x 2048 x 4096                             13.6       10.5        18.1
-//   48332 x 256 x 256                              16.4       10.5         9.9
 //   4096 x 4096 x 4096                             79.8       48.5        37.7
 //   8192 x 8192 x 8192                              540        326         258
+// with the quantisation:                  64 x 64   64 x 128   128 x 128   256 x 256
+//   512 x 4096 x 4096                       14.8       17.1        18.6        32.0
+//   1024 x 4096 x 4096                      24.7       19.1        21.4        34.3
+//   2048 x 4096 x 4096                      43.9       37.0        29.8        36.6
+//   13505 x 256 x 256 float32               11.8       10.4        10.7        14.1
+//   48332 x 256 x 256 float32                          24.4        24.6        25.9
+//   96493 x 128 x 128 float32               28.8       24.4        24.4        29.7
+//   16384 x 2048 x 1024                                49.8        44.3        42.0
+//   16384 x 2048 x 1152                                53.2        50.1        55.7
+//   8192 x 8192 x 2176                                  143         136         148
 // and experts with their quantisation, by average rows per expert:
 //                           16 columns   32 x 128   64 x 128   64 x 64   128 x 128   256 x 256
 //   32 of 2048 -> 4096:  1        20.1       22.5       20.7      20.4        29.3        41.7
@@ -814,7 +822,9 @@ int launch_raw(const ProductArgs& a, hipStream_t stream) {
 int launch_product(ProductArgs a, hipStream_t stream) {
   a.out_wide = reinterpret_cast<uintptr_t>(a.out) % 16 == 0 && a.n_out * dtype_size(a.out_dtype) % 16 == 0;
   const int64_t per_group = a.offsets ? ceil_div(a.rows, a.groups) : a.rows;
-  const auto tiles = [&](int64_t size) { return (a.rows / size + (a.offsets ? a.groups / 2 : 1)) * ceil_div(a.n_out, size); };
+  const auto tiles = [&](int64_t m, int64_t n) {
+    return (a.offsets ? a.rows / m + a.groups / 2 : ceil_div(a.rows, m)) * ceil_div(a.n_out, n);
+  };
   const int64_t expert_tiles = a.offsets ? a.groups * ceil_div(a.n_out, 128) : 0;      // if each expert's rows fit one row tile
   if (expert_tiles >= kCus && per_group >= 2 && per_group <= 96) {
     // experts have uneven numbers of rows, so 32 rows hold most of them up to an average of 12 only; where there are many tiles to hide in, of 24
@@ -829,8 +839,11 @@ int launch_product(ProductArgs a, hipStream_t stream) {
   }
   if ((ceil_div(a.rows, 32) + (a.offsets ? a.groups : 0)) * ceil_div(a.n_out, 16) <= kCus) return launch_skinny<2, 8>(a, stream);
   if (a.offsets == nullptr && a.rows <= 32) return launch_skinny<2, 4>(a, stream);
-  if (per_group >= 256 && tiles(256) >= kCus) return launch_tile<2, 4, 4, 2, 2>(a, stream);
-  if ((a.offsets || a.rows >= 96) && tiles(128) >= kCus) return launch_tile<2, 4, 2, 1, 2>(a, stream);
+  // 256 x 256 tiles go over the chip in rounds of 256 and take 1.6 times as long as 128 x 128 ones, which go in rounds of 512
+  const int64_t t256 = tiles(256, 256), t128 = tiles(128, 128), t64 = tiles(64, 128);
+  if (per_group >= 256 && t256 >= kCus && 8 * ceil_div(t256, kCus) <= 5 * ceil_div(t128, 2 * kCus)) return launch_tile<2, 4, 4, 2, 2>(a, stream);
+  if (a.n_out > 64 && t64 > kCus && t64 <= 3 * kCus) return launch_tile<2, 2, 1, 2, 2>(a, stream);     // three of them to a CU: one round
+  if ((a.offsets || a.rows >= 96) && t128 >= kCus) return launch_tile<2, 4, 2, 1, 2>(a, stream);
   return launch_tile<2, 2, 1, 1, 4>(a, stream);
 }
 

@@ -194,6 +194,28 @@ def test_dense_in_every_tile_size(amd, dtype, rows, k, n):
     _check_product(amd.mxfp4_dense(x, w4, None, None, torch.float32), x64, w64, None, False, torch.float32)
 
 
+@pytest.mark.parametrize('dtype, rows, k, n', [
+    (torch.bfloat16, 4001, 520, 4090), (torch.float32, 3990, 288, 4088), (torch.float16, 4033, 33, 4096), (torch.bfloat16, 7937, 40, 4090),  # 256 x 256
+    (torch.bfloat16, 3001, 300, 2008), (torch.float16, 13505, 96, 255), (torch.float32, 700, 520, 4001)], ids=str)      # 64 x 128
+def test_dense_in_full_rounds_of_tiles(amd, dtype, rows, k, n):
+    """Sizes whose tiles, the largest or a middling one, go over the chip at once or twice; ragged edges, an activation of its own, NaN."""
+    rng = np.random.default_rng(rows)
+    x, w = _features(rng, (rows, k), dtype), _features(rng, (n, k), torch.float32) * 0.05
+    bias = torch.as_tensor(rng.standard_normal(n), dtype=torch.float32).cuda()
+    w4 = amd.mxfp4_quantize(w)
+    x64, w64 = _plain(amd.mxfp4_quantize(x)), _plain(w4)
+    _check_product(amd.mxfp4_dense(x, w4, bias, 'relu'), x64, w64, bias.double().cpu().numpy(), True, dtype)
+    clean = amd.mxfp4_dense(x, w4, None, None, torch.float32)
+    _check_product(clean, x64, w64, None, False, torch.float32)
+    tanh = amd.mxfp4_dense(x, w4, None, 'tanh', torch.float32)
+    assert (tanh.double() - torch.tanh(clean.double())).abs().max() <= 1e-5             # the same float32 sum on both sides
+    x[rows - 1, k - 1] = float('nan')
+    w[n - 1, 0] = float('inf')
+    got = amd.mxfp4_dense(x, amd.mxfp4_quantize(w), None, None, torch.float32)
+    assert torch.isnan(got[rows - 1]).all() and torch.isnan(got[:, n - 1]).all()
+    assert torch.equal(got[:rows - 1, :n - 1], clean[:rows - 1, :n - 1])
+
+
 def test_generic_activation_in_large_tiles(amd, oracle):
     rng = np.random.default_rng(8)
     w = amd.mxfp4_quantize(_features(rng, (4104, 64), torch.float32) * 0.05)
@@ -279,9 +301,9 @@ def test_expert_dense_of_a_few_rows(amd, dtype, t, top_k, e, k, n):
 @pytest.mark.parametrize('t, top_k, e, k, n, dtype', [
     (100, 3, 40, 288, 1000, torch.bfloat16), (90, 3, 40, 520, 1001, torch.float16), (1500, 1, 64, 33, 2050, torch.float32),         # 32 x 128 tiles
     (500, 2, 64, 100, 1032, torch.float32), (3000, 1, 40, 300, 833, torch.bfloat16), (700, 3, 37, 1030, 904, torch.float16),        # 64 x 128
-    (300, 1, 5, 160, 4100, torch.bfloat16), (700, 2, 5, 64, 4100, torch.float16)], ids=str)                                        # 64 x 64, 128 x 128
+    (300, 1, 5, 160, 4100, torch.bfloat16), (700, 2, 5, 64, 4100, torch.float16), (1950, 2, 3, 160, 4090, torch.bfloat16)], ids=str)  # 64 x 64, 64 x 128, 256 x 256
 def test_expert_dense_with_some_rows_each(amd, t, top_k, e, k, n, dtype):
-    """Two to three hundred rows per expert on average, very unevenly: experts of no row, of one, of several tiles; dropped choices."""
+    """Two to a thousand rows per expert on average, very unevenly: experts of no row, of one, of several tiles; dropped choices."""
     rng = np.random.default_rng(t + n)
     share = rng.permutation(np.arange(e) ** 2 + 0.0)
     index = np.where(rng.random((t, top_k)) < 0.05, -1, rng.choice(e, (t, top_k), p=share / share.sum())).astype(np.int32)
