@@ -194,10 +194,12 @@ __global__ __launch_bounds__(kSortThreads) void k_expert_rank(const int32_t* __r
 }
 
 // What the row kernels are given.  slot[t][j] is the row of token t's choice j; a value outside 0..n-1 is a dropped choice.  A row is worked
-// on in pieces of N elements: 16 bytes where every row starts on 16 bytes.  Where they do not, dispatch and combine's gradient, which
-// write top_k rows for one they read, take pieces of the size that rows do start on (13505 x 3 rows of 333 float16: 9.8 us against 13.8
-// with unaligned 16-byte ones, 19.5 against 23.9), and combine and dispatch's gradient, which read top_k rows for one they
-// write, unaligned 16-byte ones with a short last one (FULL = false; 10.3 us against 20.7 with single elements).
+// on in pieces of N elements: 16 bytes where every row starts on 16 bytes.  Where they do not, dispatch, which writes top_k rows for one it
+// reads, takes pieces of the size that rows do start on (13505 x 3 rows of 333 float16: 9.8 us against 13.8 with unaligned 16-byte ones), and
+// combine and dispatch's gradient, which read top_k rows for one they write, unaligned 16-byte ones with a short last one (FULL = false;
+// 10.3 us against 20.7 with single elements).  Combine's gradient takes those where rows start on 4 bytes (8000 x 4 rows of 1001 float32
+// 65 us against 87 with 4-byte pieces, 30000 x 2 of 33 10.1 against 17.0, 8000 x 4 of 500 bf16 21.1 against 29.5), and single
+// elements where they start on 2 (333 float16 19.5 against 23.9).
 struct RowArgs {
   int64_t n_tokens, n_rows;
   int32_t top_k, n_experts;
@@ -342,7 +344,7 @@ __device__ __forceinline__ float sum_over_lanes(float v, int lanes) {
 // Combine's gradient: grad_rows[slot[t][j]] = weights[t][j] grad[t], grad_weights[t][j] = <grad[t], rows[slot[t][j]]>
 // (0 where the choice was dropped).  One pass: a token's gradient is read once per four choices, each choice's row read once
 // and its gradient written once.  The dot product is a float32 sum per lane, then a fixed tree over the lanes.
-template <typename T, int N, int U, bool ONCE>
+template <typename T, int N, bool FULL, int U, bool ONCE>
 __global__ __launch_bounds__(kThreads) void k_expert_combine_grad(RowArgs a, const T* __restrict__ grad, const T* __restrict__ rows,
                                                                   const float* __restrict__ weights, T* __restrict__ grad_rows,
                                                                   float* __restrict__ grad_weights) {
@@ -362,13 +364,13 @@ __global__ __launch_bounds__(kThreads) void k_expert_combine_grad(RowArgs a, con
         Pack<T, N> g[U], v[4][U];
 #pragma unroll
         for (int i = 0; i < U; ++i)
-          if (u + i * lanes < a.pieces) g[i] = load_piece<T, N, true, ONCE>(grad + t * a.width, u + i * lanes, a.width);
+          if (u + i * lanes < a.pieces) g[i] = load_piece<T, N, FULL, ONCE>(grad + t * a.width, u + i * lanes, a.width);
 #pragma unroll
         for (int j = 0; j < 4; ++j)
           if (r[j] >= 0)
 #pragma unroll
             for (int i = 0; i < U; ++i)
-              if (u + i * lanes < a.pieces) v[j][i] = load_piece<T, N, true, ONCE>(rows + r[j] * a.width, u + i * lanes, a.width);
+              if (u + i * lanes < a.pieces) v[j][i] = load_piece<T, N, FULL, ONCE>(rows + r[j] * a.width, u + i * lanes, a.width);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           if (r[j] < 0) continue;
@@ -381,7 +383,7 @@ __global__ __launch_bounds__(kThreads) void k_expert_combine_grad(RowArgs a, con
               dot[j] = fmaf(to_f32(g[i].v[c]), to_f32(v[j][i].v[c]), dot[j]);
               o.v[c] = from_f32<T>(w[j] * to_f32(g[i].v[c]));
             }
-            store_piece<T, N, true>(grad_rows + r[j] * a.width, u + i * lanes, a.width, o);
+            store_piece<T, N, FULL>(grad_rows + r[j] * a.width, u + i * lanes, a.width, o);
           }
         }
       }
@@ -448,7 +450,8 @@ int by_type(int32_t dtype, int64_t width, std::initializer_list<const void*> ptr
 
 // Rows of that many pieces are worked on two pieces a lane at a time: combine of 16384 x 4 rows of 2048 bf16 76 us against 83, of 4096 x 2 rows
 // of 1024 4.9 against 5.3 (256 float32, 64 pieces: 66 against 52); combine's gradient from twice as many on: 146 against 153, but
-// 12.3 against 9.2 at 128 pieces.
+// 12.3 against 9.2 at 128 pieces; with single elements four a lane from 400 on: 8000 x 4 rows of 1001 bf16 37.8 against 54.1, of 501 22.6 against
+// 29.8, but 13.0 against 11.0 at 201.
 constexpr int kWidePieces = 128;
 
 // Where the rows are more than the L2s hold (8 x 4 MB) everything is read past the caches, which are then left to what is written.  bf16 rows of 1 KB,
@@ -576,12 +579,12 @@ int gunet_expert_combine_grad(const void* grad_out, const void* rows, int32_t dt
   return by_type(dtype, width, {grad_out, rows, grad_rows}, [&](auto tag) {
     using Tag = decltype(tag);
     using T = typename Tag::type;
-    const RowArgs a = row_args(n_tokens, top_k, n_experts, width, Tag::vec, slot, offsets);
-    constexpr bool kFull = Tag::vec == kVec<T>;
-    constexpr int kWide = kFull ? 2 : 1;
-    const bool wide = a.pieces >= 2 * kWidePieces, once = kFull && read_once(a, dtype);
-    auto* const kernel = wide ? (once ? &k_expert_combine_grad<T, Tag::vec, kWide, kFull> : &k_expert_combine_grad<T, Tag::vec, kWide, false>)
-                              : (once ? &k_expert_combine_grad<T, Tag::vec, 1, kFull> : &k_expert_combine_grad<T, Tag::vec, 1, false>);
+    constexpr bool kFull = Tag::vec == kVec<T>, kSingle = sizeof(T) == 2 && Tag::vec == 1, kWhole = kFull || kSingle;
+    constexpr int N = kSingle ? 1 : kVec<T>, kWide = kSingle ? 4 : 2;
+    const RowArgs a = row_args(n_tokens, top_k, n_experts, width, N, slot, offsets);
+    const bool wide = a.pieces >= (kSingle ? 400 : 2 * kWidePieces), once = kFull && read_once(a, dtype);
+    auto* const kernel = wide ? (once ? &k_expert_combine_grad<T, N, kWhole, kWide, kFull> : &k_expert_combine_grad<T, N, kWhole, kWide, false>)
+                              : (once ? &k_expert_combine_grad<T, N, kWhole, 1, kFull> : &k_expert_combine_grad<T, N, kWhole, 1, false>);
     kernel<<<row_grid(a), kThreads, 0, as_stream(stream)>>>(
         a, static_cast<const T*>(grad_out), static_cast<const T*>(rows), weights, static_cast<T*>(grad_rows), grad_weights);
     GUNET_LAUNCH_CHECK();

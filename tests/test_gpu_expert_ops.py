@@ -120,6 +120,29 @@ def test_rows_there_and_back_with_gradients(amd, dtype, t, k, e, width, pattern)
     assert torch.equal(amd.expert_combine(rows, weights, plan), out)
 
 
+@pytest.mark.parametrize('dtype', TYPES, ids=str)
+@pytest.mark.parametrize('t, k, e, width, shift', [(41, 3, 5, 1001, 0), (23, 5, 4, 2050, 0), (64, 2, 3, 30, 0), (50, 4, 6, 64, 1), (19, 6, 5, 1040, 2), (70, 1, 3, 399, 0)])
+def test_combine_grad_of_rows_off_16_bytes(amd, dtype, t, k, e, width, shift):
+    """Rows that start on 4 or 2 bytes, by their width or because the tensor does; some, many and very many pieces."""
+    rng = np.random.default_rng(width)
+    plan = amd.expert_plan(torch.as_tensor(_index(rng, t, k, e, 'dropped')).cuda(), e)
+
+    def make(n):
+        v = torch.zeros(n * width + shift, dtype=dtype, device='cuda')[shift:].view(n, width)
+        v.copy_(torch.as_tensor(rng.standard_normal((n, width))))
+        return v
+
+    grad, rows = make(t), make(t * k)
+    weights = torch.as_tensor(rng.random((t, k)), dtype=torch.float32).cuda()
+    g64, r64, w64 = (v.double().cpu().numpy() for v in (grad, rows, weights))
+    want_rows, want_weights, size = R.combine_grad(g64, r64, w64, plan.slot.cpu().numpy())
+    grad_rows, grad_weights = amd.expert_combine_grad(grad, rows, weights, plan)
+    _near(grad_rows, want_rows, dtype, 1, np.abs(want_rows))
+    _near(grad_weights, want_weights, torch.float32, width, size)
+    used = int(plan.offsets[-1])
+    assert used < t * k and not grad_rows[used:].any()
+
+
 def test_gradients_against_differences(amd):
     """<c, combine(rows, w)> moved along a direction: central differences of a bilinear form are exact up to float32
     rounding of the sums, about 2^-23 of the terms' size over the step."""
