@@ -678,6 +678,122 @@ __global__ __launch_bounds__(64 * NW) void k_mxfp4_skinny(ProductArgs a) {
   }
 }
 
+// The form for small weights and any number of rows of one group: a workgroup quantises its 16 * MF rows of x into LDS and computes all their
+// columns (or every gridDim.y-th share of them), so x is read once and never written in 4 bits, and one launch does it all.  A wave takes 16
+// columns at a time over the whole K axis (v_mfma_scale_f32_16x16x128, as above), their weights from the L2s straight to registers, a turn
+// ahead.  Rows lie in LDS an odd number of 16 bytes apart, so that the 16 rows a fragment reads one block of lie on all 64 banks.
+constexpr int kRowsWaves = 8;
+template <int MF, typename XT, bool VEC, bool ANY_ACT>
+__global__ __launch_bounds__(64 * kRowsWaves) void k_mxfp4_rows(ProductArgs a) {
+  constexpr int NW = kRowsWaves;
+  extern __shared__ __attribute__((aligned(16))) char rows_smem[];      // codes [rows][pitch], scales [rows][tiles][8]
+  const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t row0 = static_cast<int64_t>(blockIdx.x) * (16 * MF);
+  const int rows = static_cast<int>(min(static_cast<int64_t>(16 * MF), a.rows - row0));
+  const uint32_t stride = static_cast<uint32_t>(a.blocks) * 16, pitch = (a.blocks | 1) * 16;
+  char* const lds_scales = rows_smem + 16 * MF * pitch;
+  const int scale_pitch = a.tiles * 8;
+  const int turns = (a.blocks + 15) / 16, sets = (a.n_out + 15) / 16, step = NW * gridDim.y;
+  struct Turn {
+    u32x4 w[4];
+    int ws;
+  };
+  const BufferRsrc wr = buffer_of(a.w_codes, static_cast<uint32_t>(a.n_out) * stride);
+  const auto fetch = [&](int set, int turn, Turn& f) __attribute__((always_inline)) {
+    const int kt = 2 * turn + (q >> 1), col = set * 16 + r;
+    f.ws = kt < a.tiles && col < a.n_out ? *reinterpret_cast<const int*>(a.w_scales + (static_cast<int64_t>(kt) * a.n_out + col) * 8 + (q & 1) * 4) : 0;
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      const int block = turn * 16 + 4 * q + s;
+      f.w[s] = __builtin_amdgcn_raw_buffer_load_b128(wr, block < a.blocks ? col * stride + block * 16 : kOutOfRange, 0, 0);
+    }
+  };
+  Turn even, odd;
+  int set = static_cast<int>(blockIdx.y) * NW + wave;
+  if (set < sets) fetch(set, 0, even);
+  const int row_parts = a.blocks * 4;
+  for (int i = threadIdx.x; i < rows * row_parts; i += 64 * NW) {
+    const int row = i / row_parts, part = i - row * row_parts, block = part >> 2;
+    uint32_t byte;
+    const uint32_t word = quantize_eight(load_eight<XT, VEC>(static_cast<const XT*>(a.x) + (row0 + row) * a.k, part * 8, a.k), &byte);
+    *reinterpret_cast<uint32_t*>(rows_smem + row * pitch + part * 4) = word;
+    char* const s8 = lds_scales + row * scale_pitch;
+    if ((part & 3) == 0) s8[block] = static_cast<char>(byte);
+    if (part == row_parts - 1)
+      for (int b = block + 1; b < scale_pitch; ++b) s8[b] = 0;
+  }
+  __syncthreads();
+  v4f acc[MF];
+#pragma unroll
+  for (int m = 0; m < MF; ++m) acc[m] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+  const auto multiply = [&](int turn, Turn& f) __attribute__((always_inline)) {
+    const int kt = 2 * turn + (q >> 1);
+#pragma unroll
+    for (int m = 0; m < MF; ++m) {
+      const int row = min(m * 16 + r, rows - 1);        // lanes of rows that are not there repeat the last one: their results are not stored
+      const int xs = kt < a.tiles ? *reinterpret_cast<const int*>(lds_scales + row * scale_pitch + kt * 8 + (q & 1) * 4) : 0;
+#pragma unroll
+      for (int s = 0; s < 4; ++s) {
+        const int block = turn * 16 + 4 * q + s;
+        const u32x4 x = block < a.blocks ? *reinterpret_cast<const u32x4*>(rows_smem + row * pitch + block * 16) : u32x4{0, 0, 0, 0};
+        acc[m] = mfma16_fp4(f.w[s], x, acc[m], s, f.ws, xs);
+      }
+    }
+  };
+  // lane (r, q) holds row r of a fragment, columns 4 q .. 4 q + 3
+  const auto columns_out = [&](int at) __attribute__((always_inline)) {
+    const int col = at * 16 + 4 * q;
+    float b[4];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) b[c] = a.bias && col + c < a.n_out ? a.bias[col + c] : 0.0f;
+#pragma unroll
+    for (int m = 0; m < MF; ++m) {
+      if (m * 16 + r < rows && col < a.n_out) {
+        const int64_t out = (row0 + m * 16 + r) * a.n_out + col;
+        float v[4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) v[c] = finish<ANY_ACT>(acc[m][c], b[c], a.act);
+        const auto four = [&](auto* p) __attribute__((always_inline)) {
+          using T = typename std::remove_pointer<decltype(p)>::type;
+          Pack<T, 4> o;
+#pragma unroll
+          for (int c = 0; c < 4; ++c) o.v[c] = from_f32<T>(v[c]);
+          store_pack<T, 4>(p + out, o);
+        };
+        if (!a.out_wide) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+            if (col + c < a.n_out) store_out(a.out, a.out_dtype, out + c, v[c]);
+        } else if (a.out_dtype == GUNET_DTYPE_F32) {
+          four(static_cast<float*>(a.out));
+        } else if (a.out_dtype == GUNET_DTYPE_BF16) {
+          four(static_cast<__bf16*>(a.out));
+        } else {
+          four(static_cast<_Float16*>(a.out));
+        }
+      }
+      acc[m] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+  };
+  int turn = 0;
+  const auto advance = [&](Turn& now, Turn& next) __attribute__((always_inline)) {
+    const int at = set, turn_now = turn;
+    if (++turn == turns) {
+      turn = 0;
+      set += step;
+    }
+    if (set < sets) fetch(set, turn, next);
+    multiply(turn_now, now);
+    if (turn == 0) columns_out(at);
+  };
+  while (set < sets) {
+    advance(even, odd);
+    if (set >= sets) break;
+    advance(odd, even);
+  }
+}
+
 // ---- host side ---------------------------------------------------------------------------------------
 
 int check_matrix(const char* fn, int64_t groups, int64_t rows, int64_t k) {
@@ -759,6 +875,38 @@ int launch_skinny(ProductArgs a, hipStream_t stream, size_t lds = 0) {
 constexpr int64_t kRawElements = 16384;
 bool raw_form(int64_t rows, int64_t k) { return rows <= 16 && rows * k <= kRawElements; }
 
+// Whether one group's product runs by rows in one launch.  Against a launch that quantises and one that multiplies (bf16, captured, us): 24 x 128 x 128
+// 3.1 / 5.0, 300 x 512 x 512 4.3 / 6.2, 1000 x 256 x 1024 4.7 / 5.9, 3410 x 128 x 128 3.5 / 5.9, 3410 x 256 x 256 4.6 / 6.0, 13505 x 256 x 256 8.4 / 9.2,
+// 24000 x 512 x 128 11.8 / 13.8, 96493 x 64 x 64 13.5 / 15.2, 96493 x 512 x 64 31.5 / 37.4; called one by one about 9 / 11.7.  Beyond, where
+// every 16 or 32 rows read all weights anew and rows are written in pieces of 16 columns: 3410 x 256 x 1024 8.6 / 7.2, 8000 x 512 x 512 11.4 / 10.4,
+// 13505 x 256 x 512 13.2 / 10.3, 48332 x 512 x 192 27.1 / 25.2, 96493 x 128 x 128 20.0 / 18.7, 300 x 2048 x 256 9.2 / 7.1.
+bool rows_form(int64_t rows, int64_t k, int64_t n_out) {
+  const bool k_fits = k <= 1024 || (k <= 2048 && rows >= 1024);
+  if (rows > 1 << 26) return false;       // one launch holds 2^32 threads
+  if (n_out <= 64) return k_fits;
+  if (n_out <= 128) return k_fits && rows <= (k <= 1024 ? 32768 : 16384);
+  if (n_out <= 256) return k <= 1024 && rows * n_out <= 3500000;
+  return n_out <= 8192 && k <= 1024 && rows * n_out <= (k <= 512 ? 512000000 : 170000000) / std::max<int64_t>(k, 128);
+}
+
+// 16 rows a workgroup and each wave 16 columns, while that makes few workgroups (or the columns are few and the quantisation is most of it); else 32, and
+// the columns shared out over what fills the chip twice.
+template <typename XT, bool VEC>
+int launch_rows(ProductArgs a, hipStream_t stream) {
+  a.out_wide = reinterpret_cast<uintptr_t>(a.out) % (4 * dtype_size(a.out_dtype)) == 0 && a.n_out % 4 == 0;
+  const int64_t shares = ceil_div(a.n_out, 16 * kRowsWaves), tiles16 = ceil_div(a.rows, 16), tiles32 = ceil_div(a.rows, 32);
+  const bool small = tiles16 * shares <= kCus * 3 / 2 || (a.n_out <= 64 && a.k >= 256 && a.k <= 1024);
+  const int64_t split = small ? shares : std::max<int64_t>(1, std::min(shares, 2 * kCus / tiles32));
+  const size_t lds = static_cast<size_t>(small ? 16 : 32) * ((a.blocks | 1) * 16 + a.tiles * 8);
+  const dim3 grid(static_cast<unsigned>(small ? tiles16 : tiles32), static_cast<unsigned>(split));
+  const bool any = !act_tuned(a.act);
+  auto* const kernel = small ? (any ? &k_mxfp4_rows<1, XT, VEC, true> : &k_mxfp4_rows<1, XT, VEC, false>)
+                             : (any ? &k_mxfp4_rows<2, XT, VEC, true> : &k_mxfp4_rows<2, XT, VEC, false>);
+  kernel<<<grid, 64 * kRowsWaves, lds, stream>>>(a);
+  GUNET_LAUNCH_CHECK();
+  return GUNET_OK;
+}
+
 // One group: sixteen waves quantise faster than eight, where they are a CU's only ones: 4 x 4096 x 1024 4.4 us against 4.8, 1 x 8192 x 1024 5.2 against
 // 5.5, 1 x 4096 x 4096 4.8 both; with two workgroups to a CU 1 x 8192 x 8192 12.8 against 11.9, 16 x 1024 x 8192 7.0 against 5.9.  (Four waves: 4 x 4096 x 1024 6.0.)
 // Experts, of which most have a row or two here: four waves, 1 token x 4 of 32 experts 2048 -> 4096 6.6 us against 8.3 with eight, and eight where
@@ -774,10 +922,12 @@ int launch_raw(const ProductArgs& a, hipStream_t stream) {
   if (a.rows * a.k > 4096 && col_tiles <= kCus) return launch_skinny<1, 16, XT, VEC>(a, stream, lds);
   return launch_skinny<1, 8, XT, VEC>(a, stream, lds);
 }
+// The forms that take x as it is: of few rows, or by rows.
 template <typename XT>
-int launch_raw(const ProductArgs& a, hipStream_t stream) {
+int launch_unquantised(const ProductArgs& a, bool raw, hipStream_t stream) {
   const bool vec = reinterpret_cast<uintptr_t>(a.x) % 16 == 0 && a.k * sizeof(XT) % 16 == 0;
-  return vec ? launch_raw<XT, true>(a, stream) : launch_raw<XT, false>(a, stream);
+  if (raw) return vec ? launch_raw<XT, true>(a, stream) : launch_raw<XT, false>(a, stream);
+  return vec ? launch_rows<XT, true>(a, stream) : launch_rows<XT, false>(a, stream);
 }
 
 // Which form.  Rows per group decide how many rows a tile can fill, the number of tiles whether they fill the chip (256 CUs).
@@ -888,10 +1038,10 @@ int run_dense(const char* fn, const void* x, int32_t dtype, int64_t x_rows, int6
     return GUNET_ERR_WORKSPACE;
   }
   GUNET_REQUIRE(need == 0 || reinterpret_cast<uintptr_t>(workspace) % 16 == 0, "%s: workspace is not 16-byte aligned", fn);
-  if (raw) {
-    if (dtype == GUNET_DTYPE_F32) return launch_raw<float>(a, stream);
-    if (dtype == GUNET_DTYPE_BF16) return launch_raw<__bf16>(a, stream);
-    return launch_raw<_Float16>(a, stream);
+  if (raw || (offsets == nullptr && rows_form(rows, k, n_out))) {
+    if (dtype == GUNET_DTYPE_F32) return launch_unquantised<float>(a, raw, stream);
+    if (dtype == GUNET_DTYPE_BF16) return launch_unquantised<__bf16>(a, raw, stream);
+    return launch_unquantised<_Float16>(a, raw, stream);
   }
   uint8_t* const x_codes = static_cast<uint8_t*>(workspace);
   GUNET_TRY(launch_quantize(x, dtype, 1, x_rows, rows, k, top_k, slot, x_codes, x_codes + codes, stream));

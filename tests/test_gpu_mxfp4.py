@@ -247,6 +247,44 @@ def test_dense_of_a_few_rows(amd, dtype, rows, k, n):
     assert torch.isnan(bad[rows - 1]).all() and torch.equal(bad[:rows - 1], got[:rows - 1])
 
 
+@pytest.mark.parametrize('dtype, rows, k, n', [
+    (torch.float32, 17, 1, 1), (torch.bfloat16, 24, 128, 8192), (torch.float16, 100, 33, 300), (torch.float32, 1000, 64, 1030), (torch.bfloat16, 3410, 128, 128),
+    (torch.float32, 3410, 256, 256), (torch.float16, 8001, 257, 250), (torch.float32, 13505, 128, 128), (torch.bfloat16, 5001, 301, 50), (torch.float16, 2000, 2048, 100),
+    (torch.float32, 4097, 1024, 64), (torch.bfloat16, 300, 512, 516), (torch.float32, 48332, 40, 7), (torch.bfloat16, 16384, 1500, 128), (torch.float16, 77, 1023, 2049)], ids=str)
+def test_dense_with_small_weights(amd, dtype, rows, k, n):
+    """The sizes of the network's own layers and around them: one launch that takes x as it is; every way of sharing out rows and columns."""
+    rng = np.random.default_rng(rows + n)
+    x, w = _features(rng, (rows, k), dtype), _features(rng, (n, k), torch.float32) * 0.05
+    bias = torch.as_tensor(rng.standard_normal(n), dtype=torch.float32).cuda()
+    w4 = amd.mxfp4_quantize(w)
+    x64, w64 = _plain(amd.mxfp4_quantize(x)), _plain(w4)
+    for out in TYPES:
+        _check_product(amd.mxfp4_dense(x, w4, bias, 'relu', out), x64, w64, bias.double().cpu().numpy(), True, out)
+    clean = amd.mxfp4_dense(x, w4, None, None, torch.float32)
+    _check_product(clean, x64, w64, None, False, torch.float32)
+    assert torch.equal(clean, amd.mxfp4_dense(x, w4, None, None, torch.float32))
+    odd = torch.zeros(rows * k + 1, dtype=dtype, device='cuda')[1:].view(rows, k)       # rows that start on no 16 bytes
+    odd.copy_(x)
+    assert torch.equal(amd.mxfp4_dense(odd, w4, None, None, torch.float32), clean)
+    tanh = amd.mxfp4_dense(x, w4, None, 'tanh', torch.float32)
+    assert (tanh.double() - torch.tanh(clean.double())).abs().max() <= 1e-5             # the same float32 sum on both sides
+    x[rows - 1, k - 1] = float('nan')
+    w[n - 1, 0] = float('inf')
+    got = amd.mxfp4_dense(x, amd.mxfp4_quantize(w), None, None, torch.float32)
+    assert torch.isnan(got[rows - 1]).all() and torch.isnan(got[:, n - 1]).all()
+    assert torch.equal(got[:rows - 1, :n - 1], clean[:rows - 1, :n - 1])
+
+
+@pytest.mark.parametrize('rows, k, n', [(300, 1100, 1000), (60, 1500, 4200), (3000, 1030, 130), (16500, 96, 255), (250, 2500, 700), (128, 1030, 8)])
+def test_dense_just_past_small_weights(amd, rows, k, n):
+    rng = np.random.default_rng(rows + n)
+    x, w4 = _features(rng, (rows, k), torch.bfloat16), amd.mxfp4_quantize(_features(rng, (n, k), torch.float32))
+    bias = torch.as_tensor(rng.standard_normal(n), dtype=torch.float32).cuda()
+    x64, w64 = _plain(amd.mxfp4_quantize(x)), _plain(w4)
+    _check_product(amd.mxfp4_dense(x, w4, bias, 'relu'), x64, w64, bias.double().cpu().numpy(), True, torch.bfloat16)
+    _check_product(amd.mxfp4_dense(x, w4, None, None, torch.float32), x64, w64, None, False, torch.float32)
+
+
 @pytest.mark.parametrize('rows, k, n', [(33, 8200, 2500), (64, 1000, 2048), (64, 1000, 2049), (90, 300, 1380), (512, 2080, 256), (512, 100, 260), (700, 32, 200)])
 def test_dense_of_a_middling_size(amd, rows, k, n):
     """Some tens to some hundreds of rows, on both sides of the size where the form of 32 rows x 16 columns no longer has a compute unit for
