@@ -436,7 +436,8 @@ int gunet_mxfp4_dequantize(const uint8_t* codes, const uint8_t* scales, int64_t 
  * then the activation, then one rounding to out_dtype.  A linear layer hands a NaN on, the ReLU of a NaN is 0
  * as in the float32 layers.  Independent of the matmul mode.  The order of the sums depends on the sizes, not on the run.
  * workspace: the quantised x, gunet_mxfp4_dense_workspace_bytes(rows, k) bytes, 16-byte aligned (0 for little x, which is
- * quantised inside the product: NULL then); calls that may overlap in time need one each. */
+ * quantised inside the product: NULL then; otherwise it is asked for whether or not these sizes use it); calls that may overlap in time
+ * need one each. */
 size_t gunet_mxfp4_dense_workspace_bytes(int64_t rows, int32_t k);
 int gunet_mxfp4_dense_forward(const void* x, int32_t dtype, int64_t rows, int32_t k, const uint8_t* w_codes,
                               const uint8_t* w_scales, const float* bias, int32_t n_out, int32_t activation, void* out,
