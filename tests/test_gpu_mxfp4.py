@@ -518,6 +518,43 @@ def test_dense_layer_in_four_bits(amd):
     _check_product(layer(x, None).view(60, 48), xq, wq, dense.bias.double().cpu().numpy(), False, torch.float32)
 
 
+def test_every_form_in_one_graph(amd):
+    """One product of each form side by side in one graph, replayed with new inputs and eager work between the replays."""
+    rng = np.random.default_rng(14)
+    sizes = [(1, 1024, 48), (5, 4000, 64), (3410, 128, 128), (100, 33, 300), (64, 2080, 80), (20, 1100, 9000), (40, 1500, 9000), (700, 1030, 4001), (3000, 33, 2056),
+             (3990, 64, 4088)]
+    xs = [torch.zeros((rows, k), dtype=torch.bfloat16, device='cuda') for rows, k, _ in sizes]
+    ws = [amd.mxfp4_quantize(_features(rng, (n, k), torch.float32)) for _, k, n in sizes]
+    shapes = [(2, 2, 8, 256, 64), (96, 2, 64, 64, 520), (900, 2, 64, 64, 520), (700, 2, 5, 64, 4100)]
+    ws += [amd.mxfp4_quantize(_features(rng, (e, n, k), torch.float32)) for _, _, e, k, n in shapes]
+    index = [torch.zeros((t, top_k), dtype=torch.int32, device='cuda') for t, top_k, *_ in shapes]
+    xs += [torch.zeros((t, k), dtype=torch.bfloat16, device='cuda') for t, _, _, k, _ in shapes]
+
+    def step():
+        out = [amd.mxfp4_dense(x, w) for x, w in zip(xs[:len(sizes)], ws)]
+        plans = [amd.expert_plan(i, shape[2]) for i, shape in zip(index, shapes)]
+        return out + [amd.mxfp4_expert_dense(x, w, p) for x, w, p in zip(xs[len(sizes):], ws[len(sizes):], plans)]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = step()
+    for turn in range(4):
+        for x in xs:
+            x.copy_(torch.as_tensor(rng.standard_normal(tuple(x.shape))))
+        for i, shape in zip(index, shapes):
+            i.copy_(torch.as_tensor(rng.integers(-1, shape[2], tuple(i.shape)).astype(np.int32)))
+        g.replay()
+        want = step()
+        assert all(torch.equal(a, b) for a, b in zip(out, want)), turn
+        assert all(a.float().abs().max() > 0 for a in out)
+
+
 def test_captured_layer_follows_new_inputs(amd):
     """Small and large products in two graphs that live together, replayed with eager work and new inputs in between."""
     rng = np.random.default_rng(13)
