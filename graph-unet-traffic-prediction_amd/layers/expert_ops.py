@@ -48,15 +48,32 @@ def checked(t, what, device=None, dtype=None, shape=None):
 
 class ExpertPlan:
     """offsets int32 [n_experts + 1] (rows of each expert), order int32 [T * k] (flat position t * k + j of each
-    row, -1 behind the last) and slot int32 [T, k] (row of each choice, -1 = dropped)."""
+    row, -1 behind the last) and slot int32 [T, k] (row of each choice, -1 = dropped).  Usually from expert_plan; parts
+    that a program has from elsewhere must be packed int32 tensors of these shapes on one GPU.  Their values are
+    taken into range by the kernels: wrong ones give wrong rows."""
 
     def __init__(self, offsets, order, slot, n_experts):
+        parts = (offsets, 'offsets'), (order, 'order'), (slot, 'slot')
+        for t, what in parts:
+            if not (isinstance(t, torch.Tensor) and t.dtype is torch.int32):
+                raise TypeError(f'{what} must be an int32 CUDA tensor')
+        if n_experts < 1 or slot.dim() != 2 or slot.shape[1] < 1:
+            raise ValueError(f'a plan is of one expert or more and slot is [T, k] with k >= 1, got {n_experts} and {tuple(slot.shape)}')
+        for (t, what), shape in zip(parts, ((n_experts + 1,), (slot.numel(),), slot.shape)):
+            if t.shape != shape or not t.is_contiguous() or t.device != slot.device:
+                raise ValueError(f'{what} must be packed {tuple(shape)} on {slot.device}, got {tuple(t.shape)} on {t.device}')
+        if not slot.is_cuda:
+            raise TypeError('the parts of a plan must be CUDA tensors')
+        self._take(offsets, order, slot, n_experts)
+
+    def _take(self, offsets, order, slot, n_experts):
         self.offsets, self.order, self.slot = offsets, order, slot
         self.n_experts = n_experts
         self.shape = slot.shape
         self.n_tokens, self.top_k = self.shape
         self.n_rows = self.n_tokens * self.top_k
         self.device = slot.device
+        return self
 
 
 def expert_plan(expert_index, n_experts):
@@ -74,7 +91,7 @@ def expert_plan(expert_index, n_experts):
     scratch = index.new_empty(nbytes // 4) if nbytes else None
     launch('gunet_expert_sort', dev, index.data_ptr(), t, k, n_experts, offsets.data_ptr(), order.data_ptr(), slot.data_ptr(),
            scratch.data_ptr() if nbytes else None, nbytes)
-    return ExpertPlan(offsets, order, slot, n_experts)
+    return ExpertPlan.__new__(ExpertPlan)._take(offsets, order, slot, n_experts)      # what __init__ checks holds by construction
 
 
 def _width(t, what, rows):
