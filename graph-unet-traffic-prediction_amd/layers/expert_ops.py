@@ -12,10 +12,12 @@ the router's weights:
 Unlike the index plans of the city graphs nothing here synchronises or is cached: a router chooses
 anew at every step, and everything can be captured into a HIP graph.  Like the rest of the package the functions record no
 autograd graph: a training step calls the gradients, `expert_combine_grad` and `expert_dispatch_grad`, itself (or from
-an autograd.Function of its own); a tensor that requires a gradient is refused rather than dropped from the graph.
+an autograd.Function of its own); a tensor that requires a gradient, or carries a forward-mode tangent, is refused rather
+than dropped from the graph.
 Tensors may be strided (they are then copied first); all of them on one GPU, whose current stream the work goes to.
 """
 import torch
+from torch.autograd import forward_ad
 
 from .. import _lib
 from .._lib import launch
@@ -43,6 +45,8 @@ def checked(t, what, device=None, dtype=None, shape=None):
     if t.requires_grad and torch.is_grad_enabled():
         raise ValueError(f'{what} requires a gradient: this call records no autograd graph (detach it, or call under '
                          'torch.no_grad() and use the _grad functions)')
+    if getattr(forward_ad, '_current_level', 0) >= 0 and forward_ad.unpack_dual(t).tangent is not None:
+        raise ValueError(f'{what} carries a tangent, which this call would drop (take forward_ad.unpack_dual({what}).primal)')
     return t if t.is_contiguous() else t.contiguous()
 
 

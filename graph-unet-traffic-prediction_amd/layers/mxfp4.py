@@ -6,7 +6,7 @@
 or, for a layer that exists already, `Mxfp4Dense.from_dense(dense)`.  Weights of several experts are one tensor [E, n_out, k],
 used by mxfp4_expert_dense on the rows that an expert_plan has sorted.  The format is OCP MXFP4: blocks of 32 columns
 share a power of two, elements are +-0, .5, 1, 1.5, 2, 3, 4, 6 (include/gunet_hip.h has every rule).  For serving: no
-gradients (a tensor that requires one is refused), nothing synchronises, everything can be captured into a HIP graph.
+gradients (a tensor that requires one or carries a tangent is refused), nothing synchronises, everything can be captured into a HIP graph.
 """
 import torch
 
