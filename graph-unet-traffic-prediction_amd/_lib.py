@@ -181,6 +181,7 @@ SIGNATURES = {
     'gunet_profile_enable': (C.c_int, [C.c_int]),
     'gunet_profile_collect': (C.c_int, [C.POINTER(F64xP), C.POINTER(I64xP), C.POINTER(F64xP)]),
     'gunet_profile_class_name': (C.c_char_p, [C.c_int]),
+    'gunet_mxfp4_form': (C.c_char_p, [C.c_int64, C.c_int32, C.c_int32, C.c_int32]),
 }
 
 

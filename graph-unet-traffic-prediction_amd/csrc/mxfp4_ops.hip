@@ -839,6 +839,20 @@ int launch_quantize(const void* x, int32_t dtype, int64_t groups, int64_t rows, 
 
 constexpr int64_t kCus = 256;     // compute units
 
+// The forms of the product: quantising x inside (kRaw*, by the number of waves), by rows (kRows*, by the rows of a workgroup), 16 columns a workgroup
+// (kSkinny*: rows, waves), tiles.
+enum Form { kRaw4, kRaw8, kRaw16, kRows16, kRows32, kSkinny16x2, kSkinny16x4, kSkinny32x4, kSkinny32x8, kTile32x128, kTile64x128, kTile64x64, kTile128x128, kTile256x256 };
+constexpr const char* kFormNames[] = {"raw 4 waves", "raw 8 waves", "raw 16 waves", "rows 16", "rows 32", "skinny 16 rows 2 waves", "skinny 16 rows 4 waves",
+                                      "skinny 32 rows 4 waves", "skinny 32 rows 8 waves", "tile 32 x 128", "tile 64 x 128", "tile 64 x 64", "tile 128 x 128",
+                                      "tile 256 x 256"};
+static_assert(sizeof(kFormNames) / sizeof(*kFormNames) == kTile256x256 + 1, "a name for each form");
+
+// What the choice of a form goes by.
+struct ProductSize {
+  int64_t rows, k, n_out;
+  int64_t groups;           // experts, or 0: one matrix for all rows
+};
+
 template <int WM, int WN, int FM, int FN, int STAGES>
 int launch_tile(ProductArgs a, hipStream_t stream) {
   using S = TileShape<WM, WN, FM, FN, STAGES>;
@@ -891,14 +905,18 @@ bool rows_form(int64_t rows, int64_t k, int64_t n_out) {
 
 // 16 rows a workgroup and each wave 16 columns, while that makes few workgroups (or the columns are few and the quantisation is most of it); else 32, and
 // the columns shared out over what fills the chip twice.
+Form choose_rows(const ProductSize& p) {
+  const bool small = ceil_div(p.rows, 16) * ceil_div(p.n_out, 16 * kRowsWaves) <= kCus * 3 / 2 || (p.n_out <= 64 && p.k >= 256 && p.k <= 1024);
+  return small ? kRows16 : kRows32;
+}
 template <typename XT, bool VEC>
-int launch_rows(ProductArgs a, hipStream_t stream) {
+int launch_rows(ProductArgs a, Form form, hipStream_t stream) {
   a.out_wide = reinterpret_cast<uintptr_t>(a.out) % (4 * dtype_size(a.out_dtype)) == 0 && a.n_out % 4 == 0;
-  const int64_t shares = ceil_div(a.n_out, 16 * kRowsWaves), tiles16 = ceil_div(a.rows, 16), tiles32 = ceil_div(a.rows, 32);
-  const bool small = tiles16 * shares <= kCus * 3 / 2 || (a.n_out <= 64 && a.k >= 256 && a.k <= 1024);
-  const int64_t split = small ? shares : std::max<int64_t>(1, std::min(shares, 2 * kCus / tiles32));
+  const bool small = form == kRows16;
+  const int64_t shares = ceil_div(a.n_out, 16 * kRowsWaves), tiles = ceil_div(a.rows, small ? 16 : 32);
+  const int64_t split = small ? shares : std::max<int64_t>(1, std::min(shares, 2 * kCus / tiles));
   const size_t lds = static_cast<size_t>(small ? 16 : 32) * ((a.blocks | 1) * 16 + a.tiles * 8);
-  const dim3 grid(static_cast<unsigned>(small ? tiles16 : tiles32), static_cast<unsigned>(split));
+  const dim3 grid(static_cast<unsigned>(tiles), static_cast<unsigned>(split));
   const bool any = !act_tuned(a.act);
   auto* const kernel = small ? (any ? &k_mxfp4_rows<1, XT, VEC, true> : &k_mxfp4_rows<1, XT, VEC, false>)
                              : (any ? &k_mxfp4_rows<2, XT, VEC, true> : &k_mxfp4_rows<2, XT, VEC, false>);
@@ -911,23 +929,24 @@ int launch_rows(ProductArgs a, hipStream_t stream) {
 // 5.5, 1 x 4096 x 4096 4.8 both; with two workgroups to a CU 1 x 8192 x 8192 12.8 against 11.9, 16 x 1024 x 8192 7.0 against 5.9.  (Four waves: 4 x 4096 x 1024 6.0.)
 // Experts, of which most have a row or two here: four waves, 1 token x 4 of 32 experts 2048 -> 4096 6.6 us against 8.3 with eight, and eight where
 // few workgroups have long rows, 1 x 2 of 8 4096 -> 4096 6.4 against 7.3; in two launches 9.1 and 8.5.
-template <typename XT, bool VEC>
-int launch_raw(const ProductArgs& a, hipStream_t stream) {
-  const size_t lds = static_cast<size_t>(a.rows) * (a.blocks * 16 + a.tiles * 8);
-  const int64_t col_tiles = ceil_div(a.n_out, 16);
-  if (a.offsets) {
-    if (a.k > 2048 && std::min<int64_t>(a.rows, a.groups + 1) * col_tiles <= 2 * kCus) return launch_skinny<1, 8, XT, VEC>(a, stream, lds);
-    return launch_skinny<1, 4, XT, VEC>(a, stream, lds);
-  }
-  if (a.rows * a.k > 4096 && col_tiles <= kCus) return launch_skinny<1, 16, XT, VEC>(a, stream, lds);
-  return launch_skinny<1, 8, XT, VEC>(a, stream, lds);
+Form choose_raw(const ProductSize& p) {
+  const int64_t col_tiles = ceil_div(p.n_out, 16);
+  if (p.groups) return p.k > 2048 && std::min<int64_t>(p.rows, p.groups + 1) * col_tiles <= 2 * kCus ? kRaw8 : kRaw4;
+  return p.rows * p.k > 4096 && col_tiles <= kCus ? kRaw16 : kRaw8;
 }
-// The forms that take x as it is: of few rows, or by rows.
+template <typename XT, bool VEC>
+int launch_raw(const ProductArgs& a, Form form, hipStream_t stream) {
+  const size_t lds = static_cast<size_t>(a.rows) * (a.blocks * 16 + a.tiles * 8);
+  if (form == kRaw4) return launch_skinny<1, 4, XT, VEC>(a, stream, lds);
+  if (form == kRaw8) return launch_skinny<1, 8, XT, VEC>(a, stream, lds);
+  return launch_skinny<1, 16, XT, VEC>(a, stream, lds);
+}
+// The forms that take x as it is.
 template <typename XT>
-int launch_unquantised(const ProductArgs& a, bool raw, hipStream_t stream) {
+int launch_unquantised(const ProductArgs& a, Form form, hipStream_t stream) {
   const bool vec = reinterpret_cast<uintptr_t>(a.x) % 16 == 0 && a.k * sizeof(XT) % 16 == 0;
-  if (raw) return vec ? launch_raw<XT, true>(a, stream) : launch_raw<XT, false>(a, stream);
-  return vec ? launch_rows<XT, true>(a, stream) : launch_rows<XT, false>(a, stream);
+  if (form <= kRaw16) return vec ? launch_raw<XT, true>(a, form, stream) : launch_raw<XT, false>(a, form, stream);
+  return vec ? launch_rows<XT, true>(a, form, stream) : launch_rows<XT, false>(a, form, stream);
 }
 
 // Which form.  Rows per group decide how many rows a tile can fill, the number of tiles whether they fill the chip (256 CUs).
@@ -969,32 +988,48 @@ int launch_unquantised(const ProductArgs& a, bool raw, hipStream_t stream) {
 // A CU takes in about 50 bytes a ns whatever the form, so a product of few tiles gains by smaller ones as long as each has a CU of its
 // own: 32 rows x 16 columns, eight waves sharing K, against 64 x 64, whole call (us): 64 x 8192 x 1024 11.6 / 16.9, 128 x 8192 x 1024 12.2 / 17.3,
 // 256 x 2048 x 512 6.8 / 8.1, 512 x 8192 x 256 16.2 / 19.9; and where there are two to a CU 128 x 8192 x 2048 20.0 / 16.8.
-int launch_product(ProductArgs a, hipStream_t stream) {
-  a.out_wide = reinterpret_cast<uintptr_t>(a.out) % 16 == 0 && a.n_out * dtype_size(a.out_dtype) % 16 == 0;
-  const int64_t per_group = a.offsets ? ceil_div(a.rows, a.groups) : a.rows;
-  const auto tiles = [&](int64_t m, int64_t n) {
-    return (a.offsets ? a.rows / m + a.groups / 2 : ceil_div(a.rows, m)) * ceil_div(a.n_out, n);
-  };
-  const int64_t expert_tiles = a.offsets ? a.groups * ceil_div(a.n_out, 128) : 0;      // if each expert's rows fit one row tile
+Form choose_quantised(const ProductSize& p) {
+  const bool experts = p.groups > 0;
+  const int64_t per_group = experts ? ceil_div(p.rows, p.groups) : p.rows;
+  const auto tiles = [&](int64_t m, int64_t n) { return (experts ? p.rows / m + p.groups / 2 : ceil_div(p.rows, m)) * ceil_div(p.n_out, n); };
+  const int64_t expert_tiles = p.groups * ceil_div(p.n_out, 128);      // if each expert's rows fit one row tile
   if (expert_tiles >= kCus && per_group >= 2 && per_group <= 96) {
     // experts have uneven numbers of rows, so 32 rows hold most of them up to an average of 12 only; where there are many tiles to hide in, of 24
-    if (per_group < 12 || (per_group <= 24 && expert_tiles >= 4 * kCus)) return launch_tile<1, 4, 1, 1, 3>(a, stream);
-    return launch_tile<2, 2, 1, 2, 2>(a, stream);
+    return per_group < 12 || (per_group <= 24 && expert_tiles >= 4 * kCus) ? kTile32x128 : kTile64x128;
   }
-  if (per_group <= (a.offsets ? 6 : 16)) {
+  if (per_group <= (experts ? 6 : 16)) {
     // two waves a workgroup stream as well as four once there are four workgroups per CU, and leave more of them side by side: 35.5 us
     // against 41.6 for 32 experts of 4 rows each
-    if (std::min<int64_t>(a.rows, a.rows / 16 + a.groups) * ceil_div(a.n_out, 16) >= 1024) return launch_skinny<1, 2>(a, stream);
-    return launch_skinny<1, 4>(a, stream);
+    return std::min<int64_t>(p.rows, p.rows / 16 + std::max<int64_t>(1, p.groups)) * ceil_div(p.n_out, 16) >= 1024 ? kSkinny16x2 : kSkinny16x4;
   }
-  if ((ceil_div(a.rows, 32) + (a.offsets ? a.groups : 0)) * ceil_div(a.n_out, 16) <= kCus) return launch_skinny<2, 8>(a, stream);
-  if (a.offsets == nullptr && a.rows <= 32) return launch_skinny<2, 4>(a, stream);
+  if ((ceil_div(p.rows, 32) + p.groups) * ceil_div(p.n_out, 16) <= kCus) return kSkinny32x8;
+  if (!experts && p.rows <= 32) return kSkinny32x4;
   // 256 x 256 tiles go over the chip in rounds of 256 and take 1.6 times as long as 128 x 128 ones, which go in rounds of 512
   const int64_t t256 = tiles(256, 256), t128 = tiles(128, 128), t64 = tiles(64, 128);
-  if (per_group >= 256 && t256 >= kCus && 8 * ceil_div(t256, kCus) <= 5 * ceil_div(t128, 2 * kCus)) return launch_tile<2, 4, 4, 2, 2>(a, stream);
-  if (a.n_out > 64 && t64 > kCus && t64 <= 3 * kCus) return launch_tile<2, 2, 1, 2, 2>(a, stream);     // three of them to a CU: one round
-  if ((a.offsets || a.rows >= 96) && t128 >= kCus) return launch_tile<2, 4, 2, 1, 2>(a, stream);
-  return launch_tile<2, 2, 1, 1, 4>(a, stream);
+  if (per_group >= 256 && t256 >= kCus && 8 * ceil_div(t256, kCus) <= 5 * ceil_div(t128, 2 * kCus)) return kTile256x256;
+  if (p.n_out > 64 && t64 > kCus && t64 <= 3 * kCus) return kTile64x128;     // three of them to a CU: one round
+  if ((experts || p.rows >= 96) && t128 >= kCus) return kTile128x128;
+  return kTile64x64;
+}
+
+Form choose_form(const ProductSize& p) {
+  if (raw_form(p.rows, p.k)) return choose_raw(p);
+  return p.groups == 0 && rows_form(p.rows, p.k, p.n_out) ? choose_rows(p) : choose_quantised(p);
+}
+
+int launch_quantised(ProductArgs a, Form form, hipStream_t stream) {
+  a.out_wide = reinterpret_cast<uintptr_t>(a.out) % 16 == 0 && a.n_out * dtype_size(a.out_dtype) % 16 == 0;
+  switch (form) {
+    case kSkinny16x2: return launch_skinny<1, 2>(a, stream);
+    case kSkinny16x4: return launch_skinny<1, 4>(a, stream);
+    case kSkinny32x4: return launch_skinny<2, 4>(a, stream);
+    case kSkinny32x8: return launch_skinny<2, 8>(a, stream);
+    case kTile32x128: return launch_tile<1, 4, 1, 1, 3>(a, stream);
+    case kTile64x128: return launch_tile<2, 2, 1, 2, 2>(a, stream);
+    case kTile64x64: return launch_tile<2, 2, 1, 1, 4>(a, stream);
+    case kTile128x128: return launch_tile<2, 4, 2, 1, 2>(a, stream);
+    default: return launch_tile<2, 4, 4, 2, 2>(a, stream);
+  }
 }
 
 int64_t align256(int64_t v) { return (v + 255) / 256 * 256; }
@@ -1031,23 +1066,23 @@ int run_dense(const char* fn, const void* x, int32_t dtype, int64_t x_rows, int6
   a.groups = groups;
   a.act = activation;
   a.out_dtype = out_dtype;
-  const bool raw = raw_form(rows, k);
-  const int64_t codes = align256(code_bytes(rows, k)), need = raw && offsets == nullptr ? 0 : codes + scale_bytes(rows, k);
+  const Form form = choose_form({rows, k, n_out, offsets ? groups : 0});
+  const int64_t codes = align256(code_bytes(rows, k)), need = form <= kRaw16 && offsets == nullptr ? 0 : codes + scale_bytes(rows, k);
   if (need > 0 && (workspace == nullptr || workspace_bytes < static_cast<size_t>(need))) {
     set_error("%s: workspace of %zu bytes, %lld are needed", fn, workspace ? workspace_bytes : size_t{0}, static_cast<long long>(need));
     return GUNET_ERR_WORKSPACE;
   }
   GUNET_REQUIRE(need == 0 || reinterpret_cast<uintptr_t>(workspace) % 16 == 0, "%s: workspace is not 16-byte aligned", fn);
-  if (raw || (offsets == nullptr && rows_form(rows, k, n_out))) {
-    if (dtype == GUNET_DTYPE_F32) return launch_unquantised<float>(a, raw, stream);
-    if (dtype == GUNET_DTYPE_BF16) return launch_unquantised<__bf16>(a, raw, stream);
-    return launch_unquantised<_Float16>(a, raw, stream);
+  if (form <= kRows32) {
+    if (dtype == GUNET_DTYPE_F32) return launch_unquantised<float>(a, form, stream);
+    if (dtype == GUNET_DTYPE_BF16) return launch_unquantised<__bf16>(a, form, stream);
+    return launch_unquantised<_Float16>(a, form, stream);
   }
   uint8_t* const x_codes = static_cast<uint8_t*>(workspace);
   GUNET_TRY(launch_quantize(x, dtype, 1, x_rows, rows, k, top_k, slot, x_codes, x_codes + codes, stream));
   a.x_codes = x_codes;
   a.x_scales = x_codes + codes;
-  return launch_product(a, stream);
+  return launch_quantised(a, form, stream);
 }
 
 }  // namespace
@@ -1111,6 +1146,11 @@ size_t gunet_mxfp4_dense_workspace_bytes(int64_t rows, int32_t k) {
 size_t gunet_mxfp4_expert_dense_workspace_bytes(int64_t rows, int32_t k) {
   if (check_matrix("mxfp4_expert_dense_workspace_bytes", 1, rows, k) != GUNET_OK) return 0;
   return static_cast<size_t>(align256(code_bytes(rows, k)) + scale_bytes(rows, k));
+}
+
+const char* gunet_mxfp4_form(int64_t rows, int32_t k, int32_t n_out, int32_t n_experts) {
+  if (check_matrix("mxfp4_form", n_experts, rows, k) != GUNET_OK || rows == 0 || n_out < 1) return "";
+  return kFormNames[choose_form({rows, k, n_out, n_experts})];
 }
 
 int gunet_mxfp4_dense_forward(const void* x, int32_t dtype, int64_t rows, int32_t k, const uint8_t* w_codes, const uint8_t* w_scales,

@@ -539,6 +539,11 @@ int gunet_profile_collect(double ms_host[GUNET_PROF_CLASSES], int64_t launches_h
                           double work_host[GUNET_PROF_CLASSES]);
 const char* gunet_profile_class_name(int cls);
 
+/* Name of the kernel form that a product on 4-bit weights of these sizes runs on: of gunet_mxfp4_dense_forward for n_experts = 0, of
+ * gunet_mxfp4_expert_dense_forward with rows = n_tokens * top_k otherwise.  A static string, "" for sizes that are refused or hold no
+ * rows; needs no GPU.  For tests and profiles: names and rules may change. */
+const char* gunet_mxfp4_form(int64_t rows, int32_t k, int32_t n_out, int32_t n_experts);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,28 @@
+"""Which form the products on 4-bit weights run on, as the library reports it (no GPU)."""
+import os
+import re
+
+import pytest
+
+from conftest import ROOT
+from mxfp4_forms import CASES, form_of
+
+
+@pytest.mark.parametrize('form, rows, k, n, experts', CASES)
+def test_sizes_run_on_their_form(form, rows, k, n, experts):
+    assert form_of(rows, k, n, experts) == form
+
+
+def test_every_form_has_sizes():
+    with open(os.path.join(ROOT, 'graph-unet-traffic-prediction_amd', 'csrc', 'mxfp4_ops.hip')) as f:
+        names = re.search(r'kFormNames\[\] = \{(.*?)\}', f.read(), re.S).group(1)
+    names = re.findall(r'"(.*?)"', names)
+    assert len(names) == 14 and set(names) == {c[0] for c in CASES}
+    # with experts there is no form by rows, and no waves to share a wider quantisation or 32 rows among
+    assert set(names) - {c[0] for c in CASES if c[4]} == {'raw 16 waves', 'rows 16', 'rows 32', 'skinny 32 rows 4 waves'}
+    assert set(names) - {c[0] for c in CASES if not c[4]} == {'raw 4 waves', 'tile 32 x 128'}
+
+
+def test_sizes_that_are_refused_have_no_form():
+    for size in ((0, 64, 8, 0), (-1, 64, 8, 0), (2 ** 31, 64, 8, 0), (4, 0, 8, 0), (4, 2 ** 22 + 1, 8, 0), (4, 64, 0, 0), (4, 64, 8, -1), (4, 64, 8, 65536)):
+        assert form_of(*size) == '', size
