@@ -252,7 +252,7 @@ __device__ __forceinline__ int count_row_tiles(const ProductArgs& a, int size) {
   for (int g = threadIdx.x & 63; g <= a.groups; g += 64) {
     int begin, end;
     group_rows(a, g, &begin, &end);
-    if (end > begin) mine += (end - begin + size - 1) / size;
+    if (end > begin) mine += (end - begin - 1) / size + 1;
   }
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) mine += __shfl_xor(mine, d);
@@ -272,7 +272,7 @@ __device__ __forceinline__ bool find_row_tile(const ProductArgs& a, int size, in
   for (int first = 0; first <= a.groups; first += 64) {
     int begin, end;
     group_rows(a, first + lane, &begin, &end);
-    const int tiles = end > begin ? (end - begin + size - 1) / size : 0;
+    const int tiles = end > begin ? (end - begin - 1) / size + 1 : 0;
     int upto = tiles;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
@@ -842,10 +842,16 @@ constexpr int64_t kCus = 256;     // compute units
 // The forms of the product: quantising x inside (kRaw*, by the number of waves), by rows (kRows*, by the rows of a workgroup), 16 columns a workgroup
 // (kSkinny*: rows, waves), tiles.
 enum Form { kRaw4, kRaw8, kRaw16, kRows16, kRows32, kSkinny16x2, kSkinny16x4, kSkinny32x4, kSkinny32x8, kTile32x128, kTile64x128, kTile64x64, kTile128x128, kTile256x256 };
-constexpr const char* kFormNames[] = {"raw 4 waves", "raw 8 waves", "raw 16 waves", "rows 16", "rows 32", "skinny 16 rows 2 waves", "skinny 16 rows 4 waves",
-                                      "skinny 32 rows 4 waves", "skinny 32 rows 8 waves", "tile 32 x 128", "tile 64 x 128", "tile 64 x 64", "tile 128 x 128",
-                                      "tile 256 x 256"};
-static_assert(sizeof(kFormNames) / sizeof(*kFormNames) == kTile256x256 + 1, "a name for each form");
+struct FormShape {
+  const char* name;
+  int rows, cols, waves;    // what a workgroup computes (kRows*: its 16 * kRowsWaves columns, at most), and its waves
+};
+constexpr FormShape kForms[] = {{"raw 4 waves", 16, 16, 4}, {"raw 8 waves", 16, 16, 8}, {"raw 16 waves", 16, 16, 16},
+                                {"rows 16", 16, 16 * kRowsWaves, kRowsWaves}, {"rows 32", 32, 16 * kRowsWaves, kRowsWaves},
+                                {"skinny 16 rows 2 waves", 16, 16, 2}, {"skinny 16 rows 4 waves", 16, 16, 4}, {"skinny 32 rows 4 waves", 32, 16, 4},
+                                {"skinny 32 rows 8 waves", 32, 16, 8}, {"tile 32 x 128", 32, 128, 4}, {"tile 64 x 128", 64, 128, 4},
+                                {"tile 64 x 64", 64, 64, 4}, {"tile 128 x 128", 128, 128, 8}, {"tile 256 x 256", 256, 256, 8}};
+static_assert(sizeof(kForms) / sizeof(*kForms) == kTile256x256 + 1, "a shape for each form");
 
 // What the choice of a form goes by.
 struct ProductSize {
@@ -853,30 +859,35 @@ struct ProductSize {
   int64_t groups;           // experts, or 0: one matrix for all rows
 };
 
-template <int WM, int WN, int FM, int FN, int STAGES>
-int launch_tile(ProductArgs a, hipStream_t stream) {
+// Workgroups of a form.  Experts: at most so many row tiles, whichever way the rows fall; what is not needed ends at once.
+int64_t form_grid(Form form, const ProductSize& p) {
+  const FormShape& f = kForms[form];
+  const int64_t row_tiles = p.groups ? std::min<int64_t>(p.rows, p.rows / f.rows + p.groups + 1) : ceil_div(p.rows, f.rows);
+  const int64_t all = row_tiles * ceil_div(p.n_out, f.cols);
+  return form >= kTile32x128 ? ceil_div(all, 8) * 8 : all;      // tiles: a run for each XCD
+}
+// Whether one launch holds them: it has less than 2^32 threads (by rows they are fewer, rows_form).
+bool form_fits(Form form, const ProductSize& p) { return form_grid(form, p) * kForms[form].waves * 64 <= UINT32_MAX; }
+
+template <Form FORM, int WM, int WN, int FM, int FN, int STAGES>
+int launch_tile(ProductArgs a, int64_t grid, hipStream_t stream) {
   using S = TileShape<WM, WN, FM, FN, STAGES>;
-  const int64_t row_tiles = a.offsets ? std::min<int64_t>(a.rows, a.rows / S::BM + a.groups + 1) : ceil_div(a.rows, S::BM);
+  static_assert(kForms[FORM].rows == S::BM && kForms[FORM].cols == S::BN && kForms[FORM].waves == S::NW, "the form's shape is the kernel's");
   a.col_tiles = static_cast<int32_t>(ceil_div(a.n_out, S::BN));
   auto* const kernel = act_tuned(a.act) ? &k_mxfp4_tile<WM, WN, FM, FN, STAGES, false> : &k_mxfp4_tile<WM, WN, FM, FN, STAGES, true>;
   if (S::kLds > (64 << 10))
     GUNET_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, S::kLds));
-  const int64_t grid = ceil_div(row_tiles * a.col_tiles, 8) * 8;
-  GUNET_REQUIRE(grid <= INT32_MAX, "mxfp4 product: %lld x %d is more than one launch holds", static_cast<long long>(a.rows), a.n_out);
   kernel<<<static_cast<unsigned>(grid), 64 * S::NW, S::kLds, stream>>>(a);
   GUNET_LAUNCH_CHECK();
   return GUNET_OK;
 }
 
-template <int MF, int NW, typename XT = void, bool VEC = false>
-int launch_skinny(ProductArgs a, hipStream_t stream, size_t lds = 0) {
-  constexpr int BM = 16 * MF;
-  const int64_t row_tiles = a.offsets ? std::min<int64_t>(a.rows, a.rows / BM + a.groups + 1) : ceil_div(a.rows, BM);
+template <Form FORM, int MF, int NW, typename XT = void, bool VEC = false>
+int launch_skinny(ProductArgs a, int64_t grid, hipStream_t stream, size_t lds = 0) {
+  static_assert(kForms[FORM].rows == 16 * MF && kForms[FORM].cols == 16 && kForms[FORM].waves == NW, "the form's shape is the kernel's");
   a.col_tiles = static_cast<int32_t>(ceil_div(a.n_out, 16));
-  GUNET_REQUIRE(row_tiles * a.col_tiles <= INT32_MAX, "mxfp4 product: %lld x %d is more than one launch holds",
-                static_cast<long long>(a.rows), a.n_out);
   auto* const kernel = act_tuned(a.act) ? &k_mxfp4_skinny<MF, NW, XT, VEC, false> : &k_mxfp4_skinny<MF, NW, XT, VEC, true>;
-  kernel<<<static_cast<unsigned>(row_tiles * a.col_tiles), 64 * NW, lds, stream>>>(a);
+  kernel<<<static_cast<unsigned>(grid), 64 * NW, lds, stream>>>(a);
   GUNET_LAUNCH_CHECK();
   return GUNET_OK;
 }
@@ -935,17 +946,17 @@ Form choose_raw(const ProductSize& p) {
   return p.rows * p.k > 4096 && col_tiles <= kCus ? kRaw16 : kRaw8;
 }
 template <typename XT, bool VEC>
-int launch_raw(const ProductArgs& a, Form form, hipStream_t stream) {
+int launch_raw(const ProductArgs& a, Form form, int64_t grid, hipStream_t stream) {
   const size_t lds = static_cast<size_t>(a.rows) * (a.blocks * 16 + a.tiles * 8);
-  if (form == kRaw4) return launch_skinny<1, 4, XT, VEC>(a, stream, lds);
-  if (form == kRaw8) return launch_skinny<1, 8, XT, VEC>(a, stream, lds);
-  return launch_skinny<1, 16, XT, VEC>(a, stream, lds);
+  if (form == kRaw4) return launch_skinny<kRaw4, 1, 4, XT, VEC>(a, grid, stream, lds);
+  if (form == kRaw8) return launch_skinny<kRaw8, 1, 8, XT, VEC>(a, grid, stream, lds);
+  return launch_skinny<kRaw16, 1, 16, XT, VEC>(a, grid, stream, lds);
 }
 // The forms that take x as it is.
 template <typename XT>
-int launch_unquantised(const ProductArgs& a, Form form, hipStream_t stream) {
+int launch_unquantised(const ProductArgs& a, Form form, int64_t grid, hipStream_t stream) {
   const bool vec = reinterpret_cast<uintptr_t>(a.x) % 16 == 0 && a.k * sizeof(XT) % 16 == 0;
-  if (form <= kRaw16) return vec ? launch_raw<XT, true>(a, form, stream) : launch_raw<XT, false>(a, form, stream);
+  if (form <= kRaw16) return vec ? launch_raw<XT, true>(a, form, grid, stream) : launch_raw<XT, false>(a, form, grid, stream);
   return vec ? launch_rows<XT, true>(a, form, stream) : launch_rows<XT, false>(a, form, stream);
 }
 
@@ -1017,18 +1028,18 @@ Form choose_form(const ProductSize& p) {
   return p.groups == 0 && rows_form(p.rows, p.k, p.n_out) ? choose_rows(p) : choose_quantised(p);
 }
 
-int launch_quantised(ProductArgs a, Form form, hipStream_t stream) {
+int launch_quantised(ProductArgs a, Form form, int64_t grid, hipStream_t stream) {
   a.out_wide = reinterpret_cast<uintptr_t>(a.out) % 16 == 0 && a.n_out * dtype_size(a.out_dtype) % 16 == 0;
   switch (form) {
-    case kSkinny16x2: return launch_skinny<1, 2>(a, stream);
-    case kSkinny16x4: return launch_skinny<1, 4>(a, stream);
-    case kSkinny32x4: return launch_skinny<2, 4>(a, stream);
-    case kSkinny32x8: return launch_skinny<2, 8>(a, stream);
-    case kTile32x128: return launch_tile<1, 4, 1, 1, 3>(a, stream);
-    case kTile64x128: return launch_tile<2, 2, 1, 2, 2>(a, stream);
-    case kTile64x64: return launch_tile<2, 2, 1, 1, 4>(a, stream);
-    case kTile128x128: return launch_tile<2, 4, 2, 1, 2>(a, stream);
-    default: return launch_tile<2, 4, 4, 2, 2>(a, stream);
+    case kSkinny16x2: return launch_skinny<kSkinny16x2, 1, 2>(a, grid, stream);
+    case kSkinny16x4: return launch_skinny<kSkinny16x4, 1, 4>(a, grid, stream);
+    case kSkinny32x4: return launch_skinny<kSkinny32x4, 2, 4>(a, grid, stream);
+    case kSkinny32x8: return launch_skinny<kSkinny32x8, 2, 8>(a, grid, stream);
+    case kTile32x128: return launch_tile<kTile32x128, 1, 4, 1, 1, 3>(a, grid, stream);
+    case kTile64x128: return launch_tile<kTile64x128, 2, 2, 1, 2, 2>(a, grid, stream);
+    case kTile64x64: return launch_tile<kTile64x64, 2, 2, 1, 1, 4>(a, grid, stream);
+    case kTile128x128: return launch_tile<kTile128x128, 2, 4, 2, 1, 2>(a, grid, stream);
+    default: return launch_tile<kTile256x256, 2, 4, 4, 2, 2>(a, grid, stream);
   }
 }
 
@@ -1066,7 +1077,10 @@ int run_dense(const char* fn, const void* x, int32_t dtype, int64_t x_rows, int6
   a.groups = groups;
   a.act = activation;
   a.out_dtype = out_dtype;
-  const Form form = choose_form({rows, k, n_out, offsets ? groups : 0});
+  const ProductSize size = {rows, k, n_out, offsets ? groups : 0};
+  const Form form = choose_form(size);
+  GUNET_REQUIRE(form_fits(form, size), "%s: %lld rows x %d columns are more than one launch holds", fn, static_cast<long long>(rows), n_out);
+  const int64_t grid = form_grid(form, size);
   const int64_t codes = align256(code_bytes(rows, k)), need = form <= kRaw16 && offsets == nullptr ? 0 : codes + scale_bytes(rows, k);
   if (need > 0 && (workspace == nullptr || workspace_bytes < static_cast<size_t>(need))) {
     set_error("%s: workspace of %zu bytes, %lld are needed", fn, workspace ? workspace_bytes : size_t{0}, static_cast<long long>(need));
@@ -1074,15 +1088,15 @@ int run_dense(const char* fn, const void* x, int32_t dtype, int64_t x_rows, int6
   }
   GUNET_REQUIRE(need == 0 || reinterpret_cast<uintptr_t>(workspace) % 16 == 0, "%s: workspace is not 16-byte aligned", fn);
   if (form <= kRows32) {
-    if (dtype == GUNET_DTYPE_F32) return launch_unquantised<float>(a, form, stream);
-    if (dtype == GUNET_DTYPE_BF16) return launch_unquantised<__bf16>(a, form, stream);
-    return launch_unquantised<_Float16>(a, form, stream);
+    if (dtype == GUNET_DTYPE_F32) return launch_unquantised<float>(a, form, grid, stream);
+    if (dtype == GUNET_DTYPE_BF16) return launch_unquantised<__bf16>(a, form, grid, stream);
+    return launch_unquantised<_Float16>(a, form, grid, stream);
   }
   uint8_t* const x_codes = static_cast<uint8_t*>(workspace);
   GUNET_TRY(launch_quantize(x, dtype, 1, x_rows, rows, k, top_k, slot, x_codes, x_codes + codes, stream));
   a.x_codes = x_codes;
   a.x_scales = x_codes + codes;
-  return launch_quantised(a, form, stream);
+  return launch_quantised(a, form, grid, stream);
 }
 
 }  // namespace
@@ -1150,7 +1164,9 @@ size_t gunet_mxfp4_expert_dense_workspace_bytes(int64_t rows, int32_t k) {
 
 const char* gunet_mxfp4_form(int64_t rows, int32_t k, int32_t n_out, int32_t n_experts) {
   if (check_matrix("mxfp4_form", n_experts, rows, k) != GUNET_OK || rows == 0 || n_out < 1) return "";
-  return kFormNames[choose_form({rows, k, n_out, n_experts})];
+  const ProductSize size = {rows, k, n_out, n_experts};
+  const Form form = choose_form(size);
+  return form_fits(form, size) ? kForms[form].name : "";
 }
 
 int gunet_mxfp4_dense_forward(const void* x, int32_t dtype, int64_t rows, int32_t k, const uint8_t* w_codes, const uint8_t* w_scales,

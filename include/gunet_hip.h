@@ -435,6 +435,7 @@ int gunet_mxfp4_dequantize(const uint8_t* codes, const uint8_t* scales, int64_t 
  * column: the transpose of a Dense kernel), n_out >= 1.  Products are exact (below 2^-126 they may be 0), sums float32; the bias (float32 [n_out] or NULL) is added last,
  * then the activation, then one rounding to out_dtype.  A linear layer hands a NaN on, the ReLU of a NaN is 0
  * as in the float32 layers.  Independent of the matmul mode.  The order of the sums depends on the sizes, not on the run.
+ * Sizes whose workgroups one launch cannot hold (2^32 threads; 2^27 results for one row, 2^36 for many) are refused.
  * workspace: the quantised x, gunet_mxfp4_dense_workspace_bytes(rows, k) bytes, 16-byte aligned (0 for little x, which is
  * quantised inside the product: NULL then; otherwise it is asked for whether or not these sizes use it); calls that may overlap in time
  * need one each. */

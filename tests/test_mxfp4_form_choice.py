@@ -15,8 +15,8 @@ def test_sizes_run_on_their_form(form, rows, k, n, experts):
 
 def test_every_form_has_sizes():
     with open(os.path.join(ROOT, 'graph-unet-traffic-prediction_amd', 'csrc', 'mxfp4_ops.hip')) as f:
-        names = re.search(r'kFormNames\[\] = \{(.*?)\}', f.read(), re.S).group(1)
-    names = re.findall(r'"(.*?)"', names)
+        table = re.search(r'kForms\[\] = (.*?);', f.read(), re.S).group(1)
+    names = re.findall(r'"(.*?)"', table)
     assert len(names) == 14 and set(names) == {c[0] for c in CASES}
     # with experts there is no form by rows, and no waves to share a wider quantisation or 32 rows among
     assert set(names) - {c[0] for c in CASES if c[4]} == {'raw 16 waves', 'rows 16', 'rows 32', 'skinny 32 rows 4 waves'}
