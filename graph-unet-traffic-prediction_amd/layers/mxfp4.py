@@ -149,7 +149,8 @@ def mxfp4_expert_dense(x, w, plan, bias=None, activation=None, out_dtype=None, s
 
 
 class Mxfp4Dense:
-    """A Dense layer served from 4-bit weights: the same call, y = activation(x @ kernel + bias)."""
+    """A Dense layer served from 4-bit weights: the same call, y = activation(x @ kernel + bias).  It can stand for in_layer or out_model
+    of a GraphUNet that has its weights, which then walks its layers one by one; loading and listing weights is the Dense layer's."""
 
     def __init__(self, units, weights, bias=None, activation=None):
         if not isinstance(weights, Mxfp4Tensor) or len(weights.shape) != 2 or weights.rows != units:

@@ -53,8 +53,8 @@ class GraphUNet(GraphBaseModel):
             self.upsampling_layers.append(us)
         self.out_model = Dense(out_units, use_bias=False, activation=output_activation)
         # call() runs the whole forward through one library call (gunet_unet_forward_f32) when the
-        # model is the plain stack of GeoQuadrantGCN layers; False walks the layer objects instead
-        # (same kernels in the same order, identical results).
+        # model is the plain stack of GeoQuadrantGCN layers between two float32 Dense layers; False walks
+        # the layer objects instead (same kernels in the same order, identical results).
         self.native_forward = True
         # True: the one-call forward keeps its intermediates in the library's static scratch buffer
         # (gunet_unet_forward_static_f32) instead of a torch-allocated workspace; graphs whose
@@ -109,6 +109,7 @@ class GraphUNet(GraphBaseModel):
         gcns = [g for _, g in self._gn_layers()]
         blocks = self.downsampling_layers + self.upsampling_layers
         return (self.native_forward and 1 <= self.depth <= _lib.MAX_DEPTH
+                and isinstance(self.in_layer, Dense) and isinstance(self.out_model, Dense)
                 and all(type(g) is GeoQuadrantGCN and g.use_global and g._act in (_lib.ACT_LINEAR, _lib.ACT_RELU)
                         for g in gcns)
                 and all(not b.residual for b in blocks)
