@@ -1,11 +1,12 @@
-"""Dense on microscaled 4-bit weights (no counterpart in the reference): the step below the bf16 matmul mode.
+"""Dense on microscaled 4-bit weights (no counterpart in the reference).
 
     w4 = mxfp4_quantize(kernel.t())                    # [n_out, k], once
     y = mxfp4_dense(x, w4, bias, 'relu')               # x is quantised on the way in
 
 or, for a layer that exists already, `Mxfp4Dense.from_dense(dense)`.  Weights of several experts are one tensor [E, n_out, k],
 used by mxfp4_expert_dense on the rows that an expert_plan has sorted.  The format is OCP MXFP4: blocks of 32 columns
-share a power of two, elements are +-0, .5, 1, 1.5, 2, 3, 4, 6 (include/gunet_hip.h has every rule).  For serving: no
+share a power of two, elements are +-0, .5, 1, 1.5, 2, 3, 4, 6 (include/gunet_hip.h has every rule).  x is rounded to 4 bits as well as the weights: on normal data a result is off by 0.16 of the
+results' root mean square, 70 times the bf16 matmul mode's 0.0024, so a network has to be made for it.  For serving: no
 gradients (a tensor that requires one or carries a tangent is refused), nothing synchronises, everything can be captured into a HIP graph.
 """
 import torch
