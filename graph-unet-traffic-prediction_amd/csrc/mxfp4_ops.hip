@@ -245,6 +245,11 @@ __device__ __forceinline__ void group_rows(const ProductArgs& a, int g, int* beg
   *end = g < a.groups ? min(max(a.offsets[g + 1], 0), rows) : rows;
 }
 
+// Row tiles that rows begin .. end - 1 are cut into (unsigned: the sum may pass 2^31).
+__device__ __forceinline__ int tiles_of(int begin, int end, int size) {
+  return end > begin ? static_cast<int>((static_cast<uint32_t>(end - begin) + size - 1) / static_cast<uint32_t>(size)) : 0;
+}
+
 // Number of row tiles of at most `size` rows that the groups' rows are cut into.
 __device__ __forceinline__ int count_row_tiles(const ProductArgs& a, int size) {
   if (a.offsets == nullptr) return static_cast<int>((a.rows + size - 1) / size);
@@ -252,7 +257,7 @@ __device__ __forceinline__ int count_row_tiles(const ProductArgs& a, int size) {
   for (int g = threadIdx.x & 63; g <= a.groups; g += 64) {
     int begin, end;
     group_rows(a, g, &begin, &end);
-    if (end > begin) mine += (end - begin - 1) / size + 1;
+    mine += tiles_of(begin, end, size);
   }
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) mine += __shfl_xor(mine, d);
@@ -272,7 +277,7 @@ __device__ __forceinline__ bool find_row_tile(const ProductArgs& a, int size, in
   for (int first = 0; first <= a.groups; first += 64) {
     int begin, end;
     group_rows(a, first + lane, &begin, &end);
-    const int tiles = end > begin ? (end - begin - 1) / size + 1 : 0;
+    const int tiles = tiles_of(begin, end, size);
     int upto = tiles;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
