@@ -337,10 +337,14 @@ __device__ __forceinline__ v16f mfma_fp4(uint4 a, uint4 b, v16f c, int step, int
 // waits for it before a barrier.  What lies out of the buffer's range reads as zeros.
 // The compiler does not look into the asm for hazards either: m0 has to be written one wait state before a load to LDS, and scalar registers
 // that the vector unit wrote (readfirstlane) five before a load that reads them.
+// m0 is a reserved register, so the compiler warns that it keeps nothing in it across the asm: nothing here asks it to.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
 __device__ __forceinline__ void dma_to_lds(u32x4 rsrc, uint32_t lds_base, uint32_t lane_off, uint32_t uniform_off) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(lds_base), "v"(lane_off), "s"(rsrc), "s"(uniform_off)
                : "memory", "m0");
 }
+#pragma clang diagnostic pop
 // Waits until at most N of this wave's loads are on their way and its LDS reads are done, then for the other waves.
 template <int N>
 __device__ __forceinline__ void wait_and_barrier() {
@@ -359,15 +363,19 @@ __device__ __forceinline__ u32x4 rsrc_of(const void* p, uint32_t bytes) {
 // flat one, which waits for the wave's stores to memory as well.
 template <typename V>
 __device__ __forceinline__ V lds_read(uint32_t at) {
-  return *(const volatile __attribute__((address_space(3))) V*)(at);
+  return *(const volatile __attribute__((address_space(3))) V*)(static_cast<uintptr_t>(at));
 }
 template <typename V>
 __device__ __forceinline__ void lds_write(uint32_t at, V v) {
-  *(volatile __attribute__((address_space(3))) V*)(at) = v;
+  *(volatile __attribute__((address_space(3))) V*)(static_cast<uintptr_t>(at)) = v;
 }
 
 constexpr int kBand = 4;
-constexpr uint32_t kOutOfRange = 0x7FFFFFF0u;   // a lane offset past every buffer here (256 rows x 512 KiB)
+// Widest rows and most columns of the form by rows (rows_form), which makes one buffer of all the weights.
+constexpr int64_t kRowsMaxK = 2048, kRowsMaxColumns = 8192;
+// A lane offset past every buffer here, and still a 32-bit one with the K axis added: a tile's 256 rows, all the columns of the form by rows.
+constexpr uint32_t kOutOfRange = 0x7FFFFFF0u;
+static_assert(256 * (kMaxK / 2) <= kOutOfRange && kRowsMaxColumns * (kRowsMaxK / 2) <= kOutOfRange && kMaxK / 2 <= UINT32_MAX - kOutOfRange, "past every buffer");
 
 // The tiled form: a workgroup of WM x WN waves computes BM rows x BN columns, a wave FM x FN fragments of 32 x 32.  K tiles of 256
 // columns (128 bytes a row, and 8 bytes of scales) go through STAGES LDS buffers, filled by direct loads STAGES - 1 tiles ahead of the
@@ -911,12 +919,12 @@ bool raw_form(int64_t rows, int64_t k) { return rows <= 16 && rows * k <= kRawEl
 // every 16 or 32 rows read all weights anew and rows are written in pieces of 16 columns: 3410 x 256 x 1024 8.6 / 7.2, 8000 x 512 x 512 11.4 / 10.4,
 // 13505 x 256 x 512 13.2 / 10.3, 48332 x 512 x 192 27.1 / 25.2, 96493 x 128 x 128 20.0 / 18.7, 300 x 2048 x 256 9.2 / 7.1.
 bool rows_form(int64_t rows, int64_t k, int64_t n_out) {
-  const bool k_fits = k <= 1024 || (k <= 2048 && rows >= 1024);
+  const bool k_fits = k <= 1024 || (k <= kRowsMaxK && rows >= 1024);
   if (rows > 1 << 26) return false;       // one launch holds 2^32 threads
   if (n_out <= 64) return k_fits;
   if (n_out <= 128) return k_fits && rows <= (k <= 1024 ? 32768 : 16384);
   if (n_out <= 256) return k <= 1024 && rows * n_out <= 3500000;
-  return n_out <= 8192 && k <= 1024 && rows * n_out <= (k <= 512 ? 512000000 : 170000000) / std::max<int64_t>(k, 128);
+  return n_out <= kRowsMaxColumns && k <= 1024 && rows * n_out <= (k <= 512 ? 512000000 : 170000000) / std::max<int64_t>(k, 128);
 }
 
 // 16 rows a workgroup and each wave 16 columns, while that makes few workgroups (or the columns are few and the quantisation is most of it); else 32, and
