@@ -64,3 +64,33 @@ def test_a_plan_from_its_parts_is_the_sorted_one():
     assert torch.equal(amd.expert_dispatch(x, made), amd.expert_dispatch(x, plan))
     empty = amd.expert_plan(index[:0], 2)
     assert amd.ExpertPlan(empty.offsets, empty.order, empty.slot, 2).n_rows == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('experts, rows, form', [(3000, 3001, 'tile 32 x 128'), (65535, 70001, 'tile 32 x 128'), (65535, 30000, 'skinny 16 rows 2 waves'),
+                                                 (65535, 9, 'raw 4 waves')])
+def test_more_experts_than_the_sort_takes(experts, rows, form):
+    """The experts' product takes 65535 of them, from a plan made by hand: rows that are in order already.  Exact sums of small whole numbers."""
+    import gunet_amd as amd
+    from mxfp4_forms import form_of
+    k, n = 64, 40
+    g = torch.Generator(device='cuda').manual_seed(rows)
+    assert form_of(rows, k, n, experts) == form
+    expert = torch.sort(torch.randint(0, experts, (rows,), generator=g, device='cuda')).values
+    expert[-1] = experts - 1
+    used = rows - 2                          # two rows belong to no expert
+    expert[:used] = torch.sort(expert[:used]).values
+    counts = torch.bincount(expert[:used], minlength=experts)
+    offsets = torch.cat([counts.new_zeros(1), counts.cumsum(0)]).to(torch.int32)
+    row = torch.arange(rows, device='cuda', dtype=torch.int32)
+    kept = torch.where(row < used, row, torch.full_like(row, -1))
+    plan = amd.ExpertPlan(offsets, kept, kept.view(rows, 1), experts)
+    level = torch.tensor([0., 1, -1, 2, -2, 3, 4, -4], device='cuda')
+    x, w = (level[torch.randint(0, 8, shape, generator=g, device='cuda')] for shape in ((rows, k), (experts, n, k)))
+    x[:, ::32], w[..., ::32] = 4, -4         # a 4 in every block: its scale is 1, and the levels stay as they are
+    bias = torch.randint(-9, 10, (experts, n), generator=g, device='cuda').float()
+    got = amd.mxfp4_expert_dense(x, amd.mxfp4_quantize(w), plan, bias)
+    want = (x[:used, None, :] * w[expert[:used]]).sum(-1) + bias[expert[:used]]
+    assert torch.equal(got[:used], want) and not got[used:].any()
+    assert torch.equal(amd.mxfp4_expert_dense(x, amd.mxfp4_quantize(w), plan, bias, sorted_rows=True)[:used], want)
+    assert torch.equal(amd.expert_dispatch(x, plan)[:used], x[:used])
