@@ -98,6 +98,12 @@ def expert_plan(expert_index, n_experts):
     return ExpertPlan.__new__(ExpertPlan)._take(offsets, order, slot, n_experts)      # what __init__ checks holds by construction
 
 
+def check_plan(plan):
+    """Its parts go to the kernels as addresses: what an ExpertPlan holds is checked, what another object holds is not."""
+    if not isinstance(plan, ExpertPlan):
+        raise TypeError(f'plan must be an ExpertPlan, got {type(plan).__name__}')
+
+
 def _width(t, what, rows):
     if t.dim() != 2 or t.shape[0] != rows:
         raise ValueError(f'{what} must be [{rows}, width], got {tuple(t.shape)}')
@@ -106,6 +112,7 @@ def _width(t, what, rows):
 
 def expert_dispatch(x, plan):
     """x [T, C] -> rows [T * k, C] in expert order (zeros behind the last expert's)."""
+    check_plan(plan)
     x = checked(x, 'x', plan.device)
     width = _width(x, 'x', plan.n_tokens)
     code = dtype_code(x, 'x')
@@ -117,6 +124,7 @@ def expert_dispatch(x, plan):
 
 def expert_dispatch_grad(grad_rows, plan):
     """Gradient of expert_dispatch: grad_rows [T * k, C] -> grad_x [T, C]."""
+    check_plan(plan)
     g = checked(grad_rows, 'grad_rows', plan.device)
     width = _width(g, 'grad_rows', plan.n_rows)
     code = dtype_code(g, 'grad_rows')
@@ -128,6 +136,7 @@ def expert_dispatch_grad(grad_rows, plan):
 
 def expert_combine(rows, weights, plan):
     """out[t] = sum_j weights[t, j] * rows[slot[t, j]]: rows [T * k, C], weights float32 [T, k] -> [T, C]."""
+    check_plan(plan)
     rows = checked(rows, 'rows', plan.device)
     width = _width(rows, 'rows', plan.n_rows)
     code = dtype_code(rows, 'rows')
@@ -140,6 +149,7 @@ def expert_combine(rows, weights, plan):
 
 def expert_combine_grad(grad_out, rows, weights, plan):
     """Gradients of expert_combine: (grad_rows [T * k, C] in the type of rows, grad_weights float32 [T, k])."""
+    check_plan(plan)
     rows = checked(rows, 'rows', plan.device)
     width = _width(rows, 'rows', plan.n_rows)
     code = dtype_code(rows, 'rows')

@@ -13,7 +13,7 @@ import torch
 
 from .. import _lib
 from .._lib import launch
-from .expert_ops import DTYPES, checked, dtype_code
+from .expert_ops import DTYPES, check_plan, checked, dtype_code
 from .hybrid_gnn import _activation_code
 
 BLOCK = 32
@@ -89,6 +89,8 @@ def mxfp4_quantize(x):
 
 def mxfp4_dequantize(t, dtype=torch.float32):
     """The values of an Mxfp4Tensor (float16 may overflow or lose the smallest ones)."""
+    if not isinstance(t, Mxfp4Tensor):
+        raise TypeError('t must be an Mxfp4Tensor')
     if dtype not in DTYPES:
         raise TypeError(f'dtype must be float32, bfloat16 or float16, got {dtype}')
     out = torch.empty(t.shape, dtype=dtype, device=t.device)
@@ -101,6 +103,7 @@ def _operands(x, w, bias, activation, out_dtype, groups_shape):
     if not isinstance(w, Mxfp4Tensor):
         raise TypeError('w must be an Mxfp4Tensor')
     x = checked(x, 'x', w.device)
+    code = dtype_code(x, 'x')
     if x.dim() < 1 or x.shape[-1] != w.k:
         raise ValueError(f'x has {x.shape[-1] if x.dim() else 0} columns, w has {w.k}')
     if bias is not None:
@@ -108,7 +111,7 @@ def _operands(x, w, bias, activation, out_dtype, groups_shape):
     out_dtype = x.dtype if out_dtype is None else out_dtype
     if out_dtype not in DTYPES:
         raise TypeError(f'out_dtype must be float32, bfloat16 or float16, got {out_dtype}')
-    return x, dtype_code(x, 'x'), bias, _activation_code(activation), out_dtype
+    return x, code, bias, _activation_code(activation), out_dtype
 
 
 def mxfp4_dense(x, w, bias=None, activation=None, out_dtype=None):
@@ -131,6 +134,7 @@ def mxfp4_expert_dense(x, w, plan, bias=None, activation=None, out_dtype=None, s
     """The experts' Dense layers on the rows of an ExpertPlan: w Mxfp4Tensor [E, n_out, k], bias float32 [E, n_out].
     x [T, k] holds the tokens (each row is dispatched in its 4-bit form), or with sorted_rows=True
     x [T * top_k, k] rows in expert order.  Returns [T * top_k, n_out] in expert order, zeros behind the last expert's rows."""
+    check_plan(plan)
     x, code, bias, act, out_dtype = _operands(x, w, bias, activation, out_dtype, (getattr(w, 'groups', 0),))
     if len(w.shape) != 3 or w.groups != plan.n_experts:
         raise ValueError(f'w must be [{plan.n_experts}, n_out, k], got {w.shape}')
