@@ -158,3 +158,54 @@ def test_every_activation_in_every_form(amd, form, rows, k, n, e):
         scale = want.abs() if name == 'exponential' else want.abs().max()
         assert torch.isfinite(want).all() and ((got - want).abs() <= 1e-5 * scale + 2.0 ** -126).all(), name
     assert not c.call(act='exponential')[c.used:].any()         # rows of no expert are zeros, not the activation of zero
+
+
+@pytest.mark.parametrize('half', [0, 1])
+def test_every_form_captured(amd, half):
+    """Products of many forms in one graph, and a second graph of the same ones: replayed in turn with new inputs and eager work in between."""
+    cases = sorted(FIRST.values(), key=str)[half::2]
+    built = [_Case(amd, *c[1:], TYPES[i % 3], _operand) for i, c in enumerate(cases)]
+    inputs = [c.x.clone() for c in built]
+
+    def step():
+        return [c.call(x, bias=True, act='relu') for c, x in zip(built, inputs)]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graphs = []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs = step()
+        graphs.append((g, outs))
+    for turn in range(4):
+        for c, x in zip(built, inputs):
+            x.copy_(c.x.roll(turn, 0) if turn % 2 else -c.x)
+        want = step()
+        for g, _ in graphs:
+            g.replay()
+        again = step()
+        torch.cuda.synchronize()
+        for i, c in enumerate(cases):
+            assert torch.equal(again[i], want[i]) and all(torch.equal(outs[i], want[i]) for _, outs in graphs), (turn, c)
+
+
+def test_every_form_on_two_streams(amd):
+    """The same products at once on two streams, each call with a workspace of its own."""
+    built = [_Case(amd, *c[1:], torch.bfloat16, _operand) for c in FIRST.values()]
+    want = [c.call() for c in built]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    for _ in range(3):
+        got = []
+        for s in streams:
+            with torch.cuda.stream(s):
+                got.append([c.call() for c in built])
+        torch.cuda.synchronize()
+        for out in got:
+            assert all(torch.equal(a, b) for a, b in zip(out, want))
+        del got, out
