@@ -1009,6 +1009,8 @@ int launch_unquantised(const ProductArgs& a, Form form, int64_t grid, hipStream_
 //    8 of 4096 -> 2048, too few tiles of 128 columns to fill the chip:
 //                        4        12.9       13.6       17.5
 //                       32                   14.2       18.0      14.0        19.4
+// Two and three rows each, where 32 x 128 begins, 16 columns / 32 x 128: 32 of 2048 -> 4096 27.0 / 29.3 and 29.8 / 30.3, 64 of 1024 -> 4096 32.4 / 28.0 and
+// 35.0 / 32.2, 64 of 1024 -> 1024 11.6 / 10.7 and 12.2 / 11.0, 128 of 512 -> 2048 28.0 / 20.9 and 29.7 / 21.5, 128 of 2048 -> 1408 36.1 / 32.8 and 38.8 / 33.7.
 // A CU takes in about 50 bytes a ns whatever the form, so a product of few tiles gains by smaller ones as long as each has a CU of its
 // own: 32 rows x 16 columns, eight waves sharing K, against 64 x 64, whole call (us): 64 x 8192 x 1024 11.6 / 16.9, 128 x 8192 x 1024 12.2 / 17.3,
 // 256 x 2048 x 512 6.8 / 8.1, 512 x 8192 x 256 16.2 / 19.9; and where there are two to a CU 128 x 8192 x 2048 20.0 / 16.8.
