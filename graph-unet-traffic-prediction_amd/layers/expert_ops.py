@@ -61,6 +61,7 @@ class ExpertPlan:
         for t, what in parts:
             if not (isinstance(t, torch.Tensor) and t.dtype is torch.int32):
                 raise TypeError(f'{what} must be an int32 CUDA tensor')
+        n_experts = int(n_experts)
         if n_experts < 1 or slot.dim() != 2 or slot.shape[1] < 1:
             raise ValueError(f'a plan is of one expert or more and slot is [T, k] with k >= 1, got {n_experts} and {tuple(slot.shape)}')
         for (t, what), shape in zip(parts, ((n_experts + 1,), (slot.numel(),), slot.shape)):

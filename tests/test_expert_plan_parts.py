@@ -1,4 +1,5 @@
 """An ExpertPlan put together by hand: its parts go to the kernels as plain addresses, so what they are is checked first."""
+import numpy as np
 import pytest
 import torch
 
@@ -56,7 +57,7 @@ def test_a_plan_from_its_parts_is_the_sorted_one():
     import gunet_amd as amd
     index = torch.tensor([[0, 1], [5, 0], [1, 1]], dtype=torch.int32, device='cuda')
     plan = amd.expert_plan(index, 2)
-    made = amd.ExpertPlan(plan.offsets.clone(), plan.order.clone(), plan.slot.clone(), 2)
+    made = amd.ExpertPlan(plan.offsets.clone(), plan.order.clone(), plan.slot.clone(), np.int64(2))
     assert {k: v for k, v in vars(made).items() if not torch.is_tensor(v)} == {k: v for k, v in vars(plan).items() if not torch.is_tensor(v)}
     for got, want in zip((made.offsets, made.order, made.slot), _parts('cuda')):
         assert torch.equal(got, want)

@@ -54,3 +54,20 @@ def test_four_bit_layers_inside_the_model(oracle):
     model.in_layer, model.out_model = in_layer, out_model
     again, _ = model(x, graph_to_dev(graph))
     assert torch.equal(again, plain)
+
+
+@pytest.mark.gpu
+def test_four_bit_layers_in_a_captured_model(oracle):
+    import gunet_amd as amd
+    from gpu_helpers import graph_to_dev, make_case, to_dev
+    x, graph, _ = make_case(oracle, 20, 24, 0.5)
+    model = _model().load_weights(oracle.make_weights(oracle.graph_unet_shapes(), 1), 'cuda')
+    model.in_layer, model.out_model = amd.Mxfp4Dense.from_dense(model.in_layer), amd.Mxfp4Dense.from_dense(model.out_model)
+    x, dev = to_dev(x, torch.float32), graph_to_dev(graph)
+    cap = amd.CapturedForward(model, x, dev)
+    for turn in range(4):
+        new = x * (1 + turn) if turn % 2 else x.roll(turn, 0)
+        got = cap(new).clone()
+        want = model.predict(new, {'edge_index': list(dev['edge_index']), 'edges': list(dev['edges']), 'node_loc': dev['node_loc'], 'global': dev['global']})
+        torch.cuda.synchronize()
+        assert torch.equal(got, want), turn
